@@ -111,7 +111,8 @@ OQ_API int oq_device_count(void);
  * error word of the library's pipelined kernels: *code = 0 when none, 1 when
  * a kernel gave up waiting on one of its internal pipeline barriers (it then
  * returned early, its outputs are undefined), 2 when oq_peer_barrier gave
- * up waiting for a peer GPU.  No reference counterpart: the reference's
+ * up waiting for a peer GPU, 3 when a 4-bit cache kernel met a page number
+ * or a position outside its arrays.  No reference counterpart: the reference's
  * Triton kernel has no internal waits.
  */
 OQ_API int oq_take_device_error(int32_t *code);
@@ -402,6 +403,137 @@ OQ_API int oq_int8_gemm(const int8_t *qx, const float *sx, const int8_t *qw,
 OQ_API int oq_int8_linear_noalloc(const void *x, int x_dtype, const int8_t *qw,
                                   const float *sw, float *y, int64_t m,
                                   int64_t n, int64_t k, oq_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * 4-bit key/value cache: rotary positions, append, read and attention.
+ * No counterpart in the reference (it quantizes weights only); the groups are
+ * its groupwise INT4 format (openquant/groupwise.py:13-61) along head_dim,
+ * with a scale that is rounded so that every cached value is an fp16 number.
+ *
+ * A paged cache of one layer: for x = k, v
+ *   x_codes  : uint8 [pages][kv_heads][page_size][head_dim / 2], two codes a
+ *              byte, element 2i in the low nibble, two's complement, -7..7
+ *   x_scales : fp16 [pages][kv_heads][page_size][head_dim / group_size]
+ *   value    = code * scale.  A group's scale is max|x| / 7 (IEEE fp32),
+ *              rounded to 8 significant bits (bf16) and kept as fp16, at most
+ *              9344 (larger magnitudes than 65408 saturate), 1 where that is
+ *              0; code = clip(rint(x / scale), -7, 7).  3 + 8 significant
+ *              bits: code * scale is exact in fp16.
+ *   A key or value that is NaN or Inf makes the keys of its token and head
+ *   read as NaN (and its values as 0): every query that sees the token gets
+ *   NaN, and no other does.
+ * All four arrays are 16-byte aligned; head_dim is 64 or 128, group_size 32,
+ * 64 or 128 and at most head_dim, page_size a multiple of 16.
+ */
+typedef struct {
+    uint8_t *k_codes;
+    void *k_scales;
+    uint8_t *v_codes;
+    void *v_scales;
+    int64_t pages;
+    int32_t page_size;
+    int32_t kv_heads;
+    int32_t head_dim;
+    int32_t group_size;
+} oq_kv4_cache;
+
+/* The sequences of one step.  Token j of sequence b is in page
+ * page_table[b * max_pages + j / page_size] at row j % page_size.  The step's
+ * own tokens are the last of each sequence: sequence b has tokens
+ * [starts[b], starts[b + 1]) of the step's arrays, at positions lengths[b] -
+ * count .. lengths[b] - 1.  starts NULL: one token per sequence, token b for
+ * sequence b.  Tokens from starts[sequences] on are padding (attention gives
+ * 0 for them, append skips them).  max_tokens is an upper bound of the tokens
+ * per sequence.  At most 2048 sequences.  All arrays int32, on the device.
+ * A page number outside the cache, a position outside the page table or the
+ * rotary table is not followed: the access is left out and the device error
+ * becomes 3 (oq_take_device_error). */
+typedef struct {
+    const int32_t *page_table;
+    const int32_t *lengths;
+    const int32_t *starts;
+    int32_t sequences;
+    int32_t max_pages;
+    int32_t max_tokens;
+} oq_kv4_batch;
+
+/* oq_rotary_spec flags: pairs (2i, 2i + 1) instead of (i, i + dim / 2), and
+ * the rotation by the negative angle (the inverse, and the gradient). */
+#define OQ_ROTARY_INTERLEAVED 1
+#define OQ_ROTARY_INVERSE 2
+
+/* table : fp32 [rows][dim], cos of the dim / 2 angles of a position, then
+ * their sin (16-byte aligned); dim even, the first dim elements of a head are
+ * rotated.  A pair (a, b) becomes (a cos - b sin, b cos + a sin), each product
+ * and sum rounded to fp32. */
+typedef struct {
+    const float *table;
+    int64_t rows;
+    int32_t dim;
+    int32_t flags;
+} oq_rotary_spec;
+
+/* Rotary positions: y = x [tokens][heads][head_dim] (fp32, fp16 or bf16,
+ * strides in elements, a head contiguous) with every token turned by its
+ * position (positions[tokens], int32, or int64 with positions_64), rounded
+ * once to x's type.  y may be x.  head_dim a multiple of 8 up to 256. */
+OQ_API int oq_rotary(const void *x, void *y, int dtype, int64_t tokens,
+                     int heads, int head_dim, int64_t x_token_stride,
+                     int64_t x_head_stride, int64_t y_token_stride,
+                     int64_t y_head_stride, const oq_rotary_spec *rotary,
+                     const void *positions, int positions_64,
+                     oq_stream_t stream);
+
+/* Writes a step's keys and values into the cache, in one kernel: k is rotated
+ * (rotary NULL: taken as it is) in fp32 and quantized without another
+ * rounding, v is quantized, and q, when not NULL, is rotated into q_out
+ * (which may be q).  k, v [tokens][kv_heads][head_dim] and q
+ * [tokens][q_heads][head_dim] are fp16 or bf16, strides in elements, a head
+ * contiguous.  positions (int32 / int64 [tokens]) replaces the tokens' places
+ * in their sequences for the rotation only; NULL: those places. */
+OQ_API int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
+                         const void *q, void *q_out, int q_heads,
+                         int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t qo_token_stride, int64_t qo_head_stride,
+                         const void *k, int64_t k_token_stride,
+                         int64_t k_head_stride, const void *v,
+                         int64_t v_token_stride, int64_t v_head_stride,
+                         int dtype, int64_t tokens,
+                         const oq_rotary_spec *rotary, const void *positions,
+                         int positions_64, oq_stream_t stream);
+
+/* What the cache holds of the step's tokens: k, v (fp16, bf16 or fp32,
+ * contiguous [tokens][kv_heads][head_dim]) = code * scale.  Padding tokens
+ * read as 0. */
+OQ_API int oq_kv4_read(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
+                       void *k, void *v, int dtype, int64_t tokens,
+                       oq_stream_t stream);
+
+/* oq_kv4_attention flag: no causal mask (every query of a sequence sees all
+ * of its tokens). */
+#define OQ_KV4_NOT_CAUSAL 1
+
+/* Attention of a step's queries over the cache: out = softmax(scale * q . K^T
+ * + mask) . V per query head, K and V the cached values of the query's
+ * sequence; query head i uses key head i / (q_heads / kv_heads).  A query at
+ * position p sees positions <= p (all with OQ_KV4_NOT_CAUSAL), and with
+ * window > 0 only those > p - window.  A row that sees nothing gives 0, and
+ * -inf as its log-sum.
+ *   q         : [tokens][q_heads][head_dim] fp16 or bf16 (strides in elements)
+ *   out       : contiguous, q's type
+ *   log_sum   : fp32 [tokens][q_heads], log sum exp(scale q.k), or NULL
+ *   workspace : oq_kv4_attention_workspace_bytes(...) bytes, 16-byte aligned,
+ *               contents ignored, in use until the work on `stream` ends */
+OQ_API int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
+                            const void *q, int dtype, int q_heads,
+                            int64_t q_token_stride, int64_t q_head_stride,
+                            void *out, float *log_sum, int64_t tokens,
+                            float scale, int64_t window, int flags,
+                            void *workspace, size_t ws_bytes,
+                            oq_stream_t stream);
+OQ_API int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache,
+                                                const oq_kv4_batch *batch,
+                                                int q_heads);
 
 #ifdef __cplusplus
 }

@@ -49,6 +49,13 @@ SIGNATURES = {
                                         _P]),
     "oq_int4_linear_host_run": (_I32, [_P, _P]),
     "oq_int4_linear_host_plan_free": (_I32, [_P]),
+    "oq_rotary": (_I32, [_P, _P, _I32, _I64, _I32, _I32, _I64, _I64, _I64, _I64, _P, _P, _I32, _P]),
+    "oq_kv4_append": (_I32, [_P, _P, _P, _P, _I32, _I64, _I64, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _I32, _I64,
+                             _P, _P, _I32, _P]),
+    "oq_kv4_read": (_I32, [_P, _P, _P, _P, _I32, _I64, _P]),
+    "oq_kv4_attention": (_I32, [_P, _P, _P, _I32, _I32, _I64, _I64, _P, _P, _I64, ctypes.c_float, _I64, _I32, _P,
+                                ctypes.c_size_t, _P]),
+    "oq_kv4_attention_workspace_bytes": (_I64, [_P, _P, _I32]),
     "oq_peer_alloc": (_I32, [ctypes.c_size_t, _P]),
     "oq_peer_free": (_I32, [_P]),
     "oq_peer_export": (_I32, [_P, _P]),

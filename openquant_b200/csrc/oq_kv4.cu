@@ -1,0 +1,555 @@
+// Rotary positions, append to and read from the 4-bit key/value cache.
+#include "oq_kv4.cuh"
+
+namespace oq {
+namespace kv4 {
+
+int check_cache(const oq_kv4_cache *c) {
+    OQ_REQUIRE(c != nullptr, "null cache");
+    OQ_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "head_dim must be 64 or 128");
+    OQ_REQUIRE(c->group_size == 32 || c->group_size == 64 || c->group_size == 128,
+               "Group size must be 32, 64 or 128");
+    OQ_REQUIRE(c->group_size <= c->head_dim, "Group size must be at most head_dim");
+    OQ_REQUIRE(c->page_size >= 16 && c->page_size % 16 == 0, "page_size must be a positive multiple of 16");
+    OQ_REQUIRE(c->pages >= 1 && c->kv_heads >= 1, "Cache dimensions must be positive");
+    // 16-row blocks are counted in 32 bits
+    OQ_REQUIRE(c->pages <= (1ll << 31) - 1 && c->pages * c->kv_heads <= (1ll << 31) / (c->page_size / 16),
+               "cache too large");
+    OQ_REQUIRE(c->k_codes && c->k_scales && c->v_codes && c->v_scales, "null pointer argument");
+    OQ_REQUIRE(aligned(c->k_codes, 16) && aligned(c->k_scales, 16) && aligned(c->v_codes, 16) &&
+                   aligned(c->v_scales, 16),
+               "cache arrays must be 16-byte aligned");
+    return OQ_OK;
+}
+
+int check_batch(const oq_kv4_batch *b, int64_t tokens) {
+    OQ_REQUIRE(b != nullptr, "null batch");
+    OQ_REQUIRE(b->sequences >= 1 && b->sequences <= kMaxSequences, "a batch has 1 to %d sequences", kMaxSequences);
+    OQ_REQUIRE(b->max_pages >= 1, "the page table needs at least one page per sequence");
+    OQ_REQUIRE(b->page_table && b->lengths, "null pointer argument");
+    OQ_REQUIRE(b->max_tokens >= 1, "max_tokens must be positive");
+    OQ_REQUIRE(tokens >= 1 && tokens < (1ll << 31), "the token count must be positive and below 2^31");
+    OQ_REQUIRE(b->starts != nullptr || b->max_tokens == 1, "max_tokens > 1 needs starts");
+    return OQ_OK;
+}
+
+namespace {
+
+constexpr int kWarps = 4;  // warps per CTA
+constexpr int kRows = 4;   // head rows a lane has in flight
+
+struct Rotary {
+    const float *table;
+    int64_t rows;
+    int dim, flags;
+    const void *positions;
+    int wide;
+};
+
+struct Rows {  // [tokens][heads][head_dim] with strides in elements
+    const void *p;
+    int64_t ts, hs;
+};
+
+__device__ __forceinline__ int64_t position_at(const Rotary &r, int64_t t) {
+    return r.wide ? __ldg(static_cast<const long long *>(r.positions) + t)
+                  : (int64_t)__ldg(static_cast<const int *>(r.positions) + t);
+}
+
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+    return __float2bfloat16_rn(v);
+}
+
+// Eight consecutive elements as fp32; VEC: 16-byte aligned.  Plain loads (not
+// the read-only path): the output may be the input.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load_row8(const T *p, float (&v)[8]) {
+    alignas(16) T e[8];
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4 *>(e)[i] = reinterpret_cast<const uint4 *>(p)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[i] = p[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f32(e[i]);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_row8(T *p, const float (&v)[8]) {
+    alignas(16) T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    if (VEC) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+            reinterpret_cast<uint4 *>(p)[i] = reinterpret_cast<const uint4 *>(e)[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = e[i];
+    }
+}
+
+// A lane's eight elements [8c, 8c + 8) of a head: the cos and signed sin that
+// each is multiplied with.  y = x cos + partner * sn, where sn carries the
+// sign of the sum's second term.
+struct Turn {
+    float cs[8], sn[8];
+    bool any;  // one of the eight is rotated
+};
+
+__device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, Turn &t) {
+    const int half = r.dim >> 1;
+    const bool inter = r.flags & OQ_ROTARY_INTERLEAVED;
+    const float sign = (r.flags & OQ_ROTARY_INVERSE) ? -1.0f : 1.0f;
+    const float *row = r.table + pos * r.dim;
+    t.any = 8 * c < r.dim;
+    if (!inter && (half & 7) == 0) {
+        if (t.any) {
+            const int i0 = 8 * c < half ? 8 * c : 8 * c - half;
+            const float s = 8 * c < half ? -sign : sign;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(row + i0) + q);
+                const float4 b = __ldg(reinterpret_cast<const float4 *>(row + half + i0) + q);
+                t.cs[4 * q] = a.x, t.cs[4 * q + 1] = a.y, t.cs[4 * q + 2] = a.z, t.cs[4 * q + 3] = a.w;
+                t.sn[4 * q] = s * b.x, t.sn[4 * q + 1] = s * b.y, t.sn[4 * q + 2] = s * b.z, t.sn[4 * q + 3] = s * b.w;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int i = 8 * c + e;
+        t.cs[e] = 1.0f;
+        t.sn[e] = 0.0f;
+        if (i < r.dim) {
+            const int a = inter ? i >> 1 : (i < half ? i : i - half);
+            const bool first = inter ? !(i & 1) : i < half;
+            t.cs[e] = __ldg(row + a);
+            t.sn[e] = (first ? -sign : sign) * __ldg(row + half + a);
+        }
+    }
+}
+
+// x cos -+ partner sin with each product and the sum rounded to fp32 (no
+// fused multiply-add): the same bits as the formula in separate operations.
+__device__ __forceinline__ float turn1(float x, float cs, float partner, float sn) {
+    return __fadd_rn(__fmul_rn(x, cs), __fmul_rn(partner, sn));
+}
+
+// Rotates a lane's eight elements.  All lanes of the warp take part; `row` is
+// the head's first element for partners that no lane's chunk lines up with.
+template <typename T>
+__device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T *row, bool active, int c, float (&x)[8]) {
+    const int half = r.dim >> 1;
+    if (r.flags & OQ_ROTARY_INTERLEAVED) {
+        if (t.any) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float a = x[e], b = x[e + 1];
+                if (8 * c + e < r.dim) {
+                    x[e] = turn1(a, t.cs[e], b, t.sn[e]);
+                    x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
+                }
+            }
+        }
+    } else if ((half & 7) == 0) {
+        const int lane = threadIdx.x & 31, step = half >> 3;
+        const int src = !t.any ? lane : (8 * c < half ? lane + step : lane - step);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const float p = __shfl_sync(0xffffffffu, x[e], src);
+            if (t.any) x[e] = turn1(x[e], t.cs[e], p, t.sn[e]);
+        }
+    } else {
+        float p[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = 8 * c + e;
+            p[e] = (active && i < r.dim) ? Elem<T>::to_f32(row[i < half ? i + half : i - half]) : 0.0f;
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (8 * c + e < r.dim) x[e] = turn1(x[e], t.cs[e], p[e], t.sn[e]);
+    }
+}
+
+// ------------------------------------------------------------- rotary ----
+//
+// HBM bound: every element is read and written once and needs 3 flops.  A
+// lane owns eight consecutive elements of a head (16 bytes of a 16-bit type),
+// head_dim / 8 lanes a head, and a warp takes kRows rounds of 32 * 8 /
+// head_dim heads of ONE token: its cos and sin are loaded once into registers
+// for all of them, and the partner of an element comes from another lane by
+// shuffle (half layout) or is the lane's own neighbour (interleaved).
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32)
+rotary_kernel(Rows x, T *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim, Rotary rot,
+              int parts) {
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t t = unit / parts;
+    if (t >= tokens) return;
+    const int lpr = head_dim >> 3, per = 32 / lpr;  // lanes a head, heads a round
+    const int sub = lane / lpr, c = lane - sub * lpr;
+    const int h0 = (int)(unit - t * parts) * kRows * per + sub;
+    const T *xt = static_cast<const T *>(x.p) + t * x.ts;
+    const int64_t pos = position_at(rot, t);
+    float v[kRows][8];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int h = h0 + i * per;
+        if (sub < per && h < heads) load_row8<T, VEC>(xt + h * x.hs + 8 * c, v[i]);
+    }
+    const bool ok = pos >= 0 && pos < rot.rows;
+    if (!ok && lane == 0) index_error();
+    Turn turn;
+    load_turn(rot, ok ? pos : 0, c, turn);
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int h = h0 + i * per;
+        rotate8<T>(rot, turn, xt + h * x.hs, sub < per && h < heads, c, v[i]);
+    }
+    __syncwarp();  // y may be x: every lane's loads (partners too) come before any store of the warp
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int h = h0 + i * per;
+        if (ok && sub < per && h < heads) store_row8<T, VEC>(y + t * y_ts + h * y_hs + 8 * c, v[i]);
+    }
+}
+
+// Place of the step's token t in its sequence, and its row of head 0 in the
+// cache (-1: none).  Returns false for a padding token.
+__device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, int64_t tokens, int64_t pages,
+                                         int page_size, int kv_heads, int64_t &pos, int64_t &at) {
+    if (seq >= bt.sequences) return false;
+    int first, count;
+    tokens_of(bt, seq, tokens, first, count);
+    if (t < first || t >= first + count) return false;
+    pos = (int64_t)length_of(bt, seq, page_size) - count + (t - first);
+    if (pos >= 0) {
+        const int page = __ldg(bt.table + (int64_t)seq * bt.max_pages + pos / page_size);
+        if (page >= 0 && page < pages) at = ((int64_t)page * kv_heads) * page_size + pos % page_size;
+    }
+    if (at < 0 && (threadIdx.x & 31) == 0) index_error();
+    return true;
+}
+
+// ------------------------------------------------------------- append ----
+//
+// HBM bound at many tokens, latency bound at a few.  The same lane layout as
+// the rotary kernel, over the token's query heads and then its key and value
+// heads in pairs (k0 v0 k1 v1 ...), so that a key and the value that goes
+// with it sit in neighbouring lane groups of one round.  A group's maximum
+// is a shuffle over group / 8 lanes; a lane's eight codes are one word.
+struct AppendArgs {
+    Rows q, k, v;
+    void *q_out;
+    int64_t qo_ts, qo_hs;
+    int q_heads, kv_heads, page_size, group_log;  // log2(group / 8): lanes a group
+    uint32_t *k_codes, *v_codes;
+    __half *k_scales, *v_scales;
+    int64_t pages, tokens;
+    int parts, q_rounds;
+    Rotary rot;  // table nullptr: no rotation
+    Batch batch;
+};
+
+template <typename T, int D, bool VEC>
+__global__ void __launch_bounds__(kWarps * 32) append_kernel(AppendArgs a) {
+    constexpr int LPR = D / 8, PER = 32 / LPR;
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t t = unit / a.parts;
+    if (t >= a.tokens) return;
+    const int sub = lane / LPR, c = lane % LPR;
+    const int round0 = (int)(unit - t * a.parts) * kRows;
+    const int kv_rows = 2 * a.kv_heads;
+
+    // row of round i: [0, q_heads) a query head; a key or value head after
+    // the rounds of the queries
+    float x[kRows][8];
+    const T *src[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int round = round0 + i;
+        src[i] = nullptr;
+        if (round < a.q_rounds) {
+            const int h = round * PER + sub;
+            if (h < a.q_heads) src[i] = static_cast<const T *>(a.q.p) + t * a.q.ts + h * a.q.hs;
+        } else {
+            const int row = (round - a.q_rounds) * PER + sub;
+            if (row < kv_rows) {
+                const Rows &m = (row & 1) ? a.v : a.k;
+                src[i] = static_cast<const T *>(m.p) + t * m.ts + (row >> 1) * m.hs;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+        if (src[i] != nullptr) load_row8<T, VEC>(src[i] + 8 * c, x[i]);
+    }
+
+    const int seq = sequence_of(a.batch, (int)t);
+    int64_t pos = 0, at = -1;  // place in the sequence; row of head 0 in the cache
+    const bool real = find_row(a.batch, seq, t, a.tokens, a.pages, a.page_size, a.kv_heads, pos, at);
+    int64_t angle = a.rot.positions != nullptr ? position_at(a.rot, t) : pos;
+    const bool turned = a.rot.table != nullptr;
+    const bool ok = !turned || (angle >= 0 && angle < a.rot.rows);
+    if (!ok && real && lane == 0) index_error();
+    Turn turn;
+    if (turned) load_turn(a.rot, ok ? angle : 0, c, turn);
+
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int round = round0 + i;
+        if (round < a.q_rounds) {  // warp-uniform
+            if (turned) rotate8<T>(a.rot, turn, src[i], src[i] != nullptr, c, x[i]);
+            __syncwarp();  // q_out may be q
+            if (src[i] != nullptr && ok)
+                store_row8<T, VEC>(static_cast<T *>(a.q_out) + t * a.qo_ts + (round * PER + sub) * a.qo_hs + 8 * c,
+                                   x[i]);
+            continue;
+        }
+        const int row = (round - a.q_rounds) * PER + sub;
+        const bool is_v = row & 1;
+        if (turned) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[i][e];
+            rotate8<T>(a.rot, turn, src[i], src[i] != nullptr, c, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[i][e] = is_v ? x[i][e] : y[e];
+        }
+        float mx = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx = nan_max(mx, fabsf(x[i][e]));
+        // Not finite anywhere in the token's key or value of this head: the
+        // lanes of both (2 * LPR of them) agree on it.
+        const unsigned bad_lanes = __ballot_sync(0xffffffffu, !(mx <= 3.402823466e38f));
+        const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
+        const bool bad = (bad_lanes & pair) != 0;
+        for (int o = 0; o < a.group_log; ++o) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
+        __half s16 = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(mx, 7.0f))));
+        float s = fminf(__half2float(s16), kMaxScale);
+        if (s == 0.0f || bad) s = 1.0f;
+        const float inv = __fdiv_rn(1.0f, s);
+        uint32_t word = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) word |= (quant_bits(x[i][e], s, inv, 7.0f) & 15u) << (4 * e);
+        if (bad) word = 0;
+        if (row < kv_rows && at >= 0 && ok) {
+            const int64_t r = at + (int64_t)(row >> 1) * a.page_size;
+            (is_v ? a.v_codes : a.k_codes)[r * (D / 8) + c] = word;
+            if ((c & ((1 << a.group_log) - 1)) == 0)
+                (is_v ? a.v_scales : a.k_scales)[r * (LPR >> a.group_log) + (c >> a.group_log)] =
+                    bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
+        }
+    }
+}
+
+// --------------------------------------------------------------- read ----
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kWarps * 32)
+read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_codes, const __half *v_scales, T *k,
+            T *v, Batch batch, int64_t pages, int page_size, int kv_heads, int group_log, int64_t tokens, int parts) {
+    constexpr int LPR = D / 8, PER = 32 / LPR;
+    const int lane = threadIdx.x & 31;
+    const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+    const int64_t t = unit / parts;
+    if (t >= tokens) return;
+    const int sub = lane / LPR, c = lane % LPR;
+    const int seq = sequence_of(batch, (int)t);
+    int64_t pos = 0, at = -1;
+    find_row(batch, seq, t, tokens, pages, page_size, kv_heads, pos, at);
+    const int row0 = (int)(unit - t * parts) * kRows * PER + sub;
+    uint32_t word[kRows];
+    __half sc[kRows];
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int row = row0 + i * PER;
+        word[i] = 0;
+        sc[i] = __ushort_as_half(0);
+        if (at >= 0 && row < 2 * kv_heads) {
+            const int64_t r = at + (int64_t)(row >> 1) * page_size;
+            word[i] = ((row & 1) ? v_codes : k_codes)[r * (D / 8) + c];
+            sc[i] = ((row & 1) ? v_scales : k_scales)[r * (LPR >> group_log) + (c >> group_log)];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int row = row0 + i * PER;
+        if (row >= 2 * kv_heads) continue;
+        const float s = __half2float(sc[i]);
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = (float)nibble_value(word[i] >> (8 * (e >> 1)), e & 1) * s;
+        store_row8<T, true>(((row & 1) ? v : k) + ((int64_t)t * kv_heads + (row >> 1)) * D + 8 * c, o);
+    }
+}
+
+int check_rotary(const oq_rotary_spec *r, int head_dim) {
+    OQ_REQUIRE(r->table != nullptr && aligned(r->table, 16), "the rotary table must be a 16-byte aligned array");
+    OQ_REQUIRE(r->rows >= 1, "the rotary table is empty");
+    OQ_REQUIRE(r->dim >= 2 && r->dim % 2 == 0 && r->dim <= head_dim,
+               "the rotary dimension must be even, at least 2 and at most head_dim");
+    OQ_REQUIRE((r->flags & ~(OQ_ROTARY_INTERLEAVED | OQ_ROTARY_INVERSE)) == 0, "unknown rotary flags");
+    return OQ_OK;
+}
+
+int grid_of(int64_t units, int64_t *blocks) {
+    *blocks = cdiv(units, kWarps);
+    OQ_REQUIRE(*blocks < (1ll << 31), "too many tokens and heads for one call");
+    return OQ_OK;
+}
+
+template <typename T>
+int rotary_launch(const Rows &x, void *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim,
+                  const Rotary &rot, cudaStream_t st) {
+    const int per = 32 / (head_dim / 8);
+    const int parts = (int)cdiv(heads, kRows * per);
+    int64_t blocks;
+    if (int rc = grid_of(tokens * parts, &blocks)) return rc;
+    const int64_t n = 16 / sizeof(T);
+    const bool vec = aligned(x.p, 16) && aligned(y, 16) && x.ts % n == 0 && x.hs % n == 0 && y_ts % n == 0 &&
+                     y_hs % n == 0;
+    if (vec)
+        rotary_kernel<T, true><<<(unsigned)blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens,
+                                                                         heads, head_dim, rot, parts);
+    else
+        rotary_kernel<T, false><<<(unsigned)blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens,
+                                                                          heads, head_dim, rot, parts);
+    return check_launch("rotary");
+}
+
+template <typename T, int D>
+int append_launch(const AppendArgs &a, bool vec, int64_t blocks, cudaStream_t st) {
+    if (vec)
+        append_kernel<T, D, true><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a);
+    else
+        append_kernel<T, D, false><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a);
+    return check_launch("kv4_append");
+}
+
+template <typename T, int D>
+int read_launch(const oq_kv4_cache *c, const Batch &b, void *k, void *v, int group_log, int64_t tokens, int parts,
+                int64_t blocks, cudaStream_t st) {
+    read_kernel<T, D><<<(unsigned)blocks, kWarps * 32, 0, st>>>(
+        reinterpret_cast<const uint32_t *>(c->k_codes), static_cast<const __half *>(c->k_scales),
+        reinterpret_cast<const uint32_t *>(c->v_codes), static_cast<const __half *>(c->v_scales), static_cast<T *>(k),
+        static_cast<T *>(v), b, c->pages, c->page_size, c->kv_heads, group_log, tokens, parts);
+    return check_launch("kv4_read");
+}
+
+int group_log_of(int group) { return group == 32 ? 2 : group == 64 ? 3 : 4; }
+
+}  // namespace
+}  // namespace kv4
+}  // namespace oq
+
+using namespace oq;
+using namespace oq::kv4;
+
+extern "C" int oq_rotary(const void *x, void *y, int dtype, int64_t tokens, int heads, int head_dim,
+                         int64_t x_token_stride, int64_t x_head_stride, int64_t y_token_stride, int64_t y_head_stride,
+                         const oq_rotary_spec *rotary, const void *positions, int positions_64, oq_stream_t stream) {
+    clear_error();
+    OQ_REQUIRE(dtype == OQ_F32 || dtype == OQ_F16 || dtype == OQ_BF16, "rotary: x must be fp32, fp16 or bf16");
+    OQ_REQUIRE(tokens >= 1 && heads >= 1, "rotary: dimensions must be positive");
+    OQ_REQUIRE(head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0,
+               "rotary: head_dim must be a multiple of 8 up to 256");
+    OQ_REQUIRE(x && y && rotary && positions, "null pointer argument");
+    if (int rc = check_rotary(rotary, head_dim)) return rc;
+    const Rows r{x, x_token_stride, x_head_stride};
+    const Rotary rot{rotary->table, rotary->rows, rotary->dim, rotary->flags, positions, positions_64};
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == OQ_F32)
+        return rotary_launch<float>(r, y, y_token_stride, y_head_stride, tokens, heads, head_dim, rot, st);
+    if (dtype == OQ_F16)
+        return rotary_launch<__half>(r, y, y_token_stride, y_head_stride, tokens, heads, head_dim, rot, st);
+    return rotary_launch<__nv_bfloat16>(r, y, y_token_stride, y_head_stride, tokens, heads, head_dim, rot, st);
+}
+
+extern "C" int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batch, const void *q, void *q_out,
+                             int q_heads, int64_t q_token_stride, int64_t q_head_stride, int64_t qo_token_stride,
+                             int64_t qo_head_stride, const void *k, int64_t k_token_stride, int64_t k_head_stride,
+                             const void *v, int64_t v_token_stride, int64_t v_head_stride, int dtype, int64_t tokens,
+                             const oq_rotary_spec *rotary, const void *positions, int positions_64,
+                             oq_stream_t stream) {
+    clear_error();
+    OQ_REQUIRE(dtype == OQ_F16 || dtype == OQ_BF16, "kv4_append: k and v must be fp16 or bf16");
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, tokens)) return rc;
+    OQ_REQUIRE(k && v, "null pointer argument");
+    OQ_REQUIRE(q == nullptr || (q_out != nullptr && q_heads >= 1), "kv4_append: q needs q_out and its head count");
+    if (rotary != nullptr)
+        if (int rc = check_rotary(rotary, cache->head_dim)) return rc;
+    AppendArgs a = {};
+    a.q = Rows{q, q_token_stride, q_head_stride};
+    a.k = Rows{k, k_token_stride, k_head_stride};
+    a.v = Rows{v, v_token_stride, v_head_stride};
+    a.q_out = q_out;
+    a.qo_ts = qo_token_stride;
+    a.qo_hs = qo_head_stride;
+    a.q_heads = q != nullptr ? q_heads : 0;
+    a.kv_heads = cache->kv_heads;
+    a.page_size = cache->page_size;
+    a.group_log = group_log_of(cache->group_size);
+    a.k_codes = reinterpret_cast<uint32_t *>(cache->k_codes);
+    a.v_codes = reinterpret_cast<uint32_t *>(cache->v_codes);
+    a.k_scales = static_cast<__half *>(cache->k_scales);
+    a.v_scales = static_cast<__half *>(cache->v_scales);
+    a.pages = cache->pages;
+    a.tokens = tokens;
+    const int per = 32 / (cache->head_dim / 8);
+    a.q_rounds = (int)cdiv(a.q_heads, per);
+    a.parts = (int)cdiv(a.q_rounds + cdiv(2 * a.kv_heads, per), kRows);
+    if (rotary != nullptr)
+        a.rot = Rotary{rotary->table, rotary->rows, rotary->dim, rotary->flags, positions, positions_64};
+    a.batch = device_batch(batch);
+    auto ok = [](const void *p, int64_t ts, int64_t hs) { return aligned(p, 16) && ts % 8 == 0 && hs % 8 == 0; };
+    const bool vec = ok(k, k_token_stride, k_head_stride) && ok(v, v_token_stride, v_head_stride) &&
+                     (q == nullptr || (ok(q, q_token_stride, q_head_stride) &&
+                                       ok(q_out, qo_token_stride, qo_head_stride)));
+    int64_t blocks;
+    if (int rc = grid_of(tokens * a.parts, &blocks)) return rc;
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == OQ_F16)
+        return cache->head_dim == 64 ? append_launch<__half, 64>(a, vec, blocks, st)
+                                     : append_launch<__half, 128>(a, vec, blocks, st);
+    return cache->head_dim == 64 ? append_launch<__nv_bfloat16, 64>(a, vec, blocks, st)
+                                 : append_launch<__nv_bfloat16, 128>(a, vec, blocks, st);
+}
+
+extern "C" int oq_kv4_read(const oq_kv4_cache *cache, const oq_kv4_batch *batch, void *k, void *v, int dtype,
+                           int64_t tokens, oq_stream_t stream) {
+    clear_error();
+    OQ_REQUIRE(dtype == OQ_F32 || dtype == OQ_F16 || dtype == OQ_BF16, "kv4_read: output must be fp32, fp16 or bf16");
+    if (int rc = check_cache(cache)) return rc;
+    if (int rc = check_batch(batch, tokens)) return rc;
+    OQ_REQUIRE(k && v, "null pointer argument");
+    OQ_REQUIRE(aligned(k, 16) && aligned(v, 16), "kv4_read: k and v must be 16-byte aligned");
+    const int per = 32 / (cache->head_dim / 8);
+    const int parts = (int)cdiv(2 * cache->kv_heads, kRows * per);
+    int64_t blocks;
+    if (int rc = grid_of(tokens * parts, &blocks)) return rc;
+    const int gl = group_log_of(cache->group_size);
+    const Batch b = device_batch(batch);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const bool d64 = cache->head_dim == 64;
+    if (dtype == OQ_F32)
+        return d64 ? read_launch<float, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
+                   : read_launch<float, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
+    if (dtype == OQ_F16)
+        return d64 ? read_launch<__half, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
+                   : read_launch<__half, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
+    return d64 ? read_launch<__nv_bfloat16, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
+               : read_launch<__nv_bfloat16, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
+}
