@@ -14,10 +14,9 @@
 // a score passes m + 14 (a warp vote per 16 tokens), which is rare after the
 // first tokens, so the maximum costs no shuffles in the steady state.
 //
-// Queries in bf16 go to fp16 times a power of two per row, exact but for
-// elements 2^-22 below the row's largest (their low bits then fall under
-// fp16's smallest step): one kernel for both types.
-#include "oq_kv4.cuh"
+// Queries in bf16 go to fp16 times a power of two per row (fp16_power): one
+// kernel for both types.
+#include "oq_kv4_attention.cuh"
 
 namespace oq {
 namespace kv4 {
@@ -26,28 +25,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kTile = 16 * kWarps;  // cached tokens of one round of a CTA
 constexpr int kStages = 4;          // 16-token stages a warp has in flight or in use
-constexpr float kLift = 6.0f;       // m = maximum - kLift
-constexpr float kRaise = 14.0f;     // m is raised when a score passes m + kRaise
 
-struct Args {
-    const uint8_t *k_codes, *v_codes;
-    const __half *k_scales, *v_scales;
-    int64_t pages;
-    int page_size, kv_heads;
-    Batch batch;
-    const void *q;
-    int64_t q_ts, q_hs;
-    void *out;
-    float *log_sum;
-    int64_t tokens;
-    int q_heads, ratio;  // ratio: query heads a key head
-    float f;             // scale * log2 e
-    int64_t window;
-    int causal;
-    float *parts;      // partial results: two slots a CTA
-    int64_t *prefix;   // units before each sequence, written by CTA 0 for the joining kernel
-    int vec;           // q rows 16-byte aligned
-};
+using Args = AttnArgs;
 
 // Columns (query rows) of a partial, and its floats: m[cols], l[cols], o[cols][HD].
 template <int HD, int NT>
@@ -71,7 +50,7 @@ __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
     tokens_of(a.batch, b, a.tokens, w.first, w.count);
     w.length = length_of(a.batch, b, a.page_size);
     w.rows = w.count * a.ratio;
-    w.blocks = (w.rows + cols - 1) / cols;
+    w.blocks = w.rows > a.few ? 0 : (w.rows + cols - 1) / cols;
     w.floor = 0;
     if (a.window > 0) w.floor = max((int64_t)w.length - w.count + 1 - a.window, (int64_t)0);
     w.lo = w.floor / kTile * kTile;
@@ -107,34 +86,6 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-template <typename T>
-__device__ __forceinline__ void put(T *p, float v);
-template <> __device__ __forceinline__ void put<__half>(__half *p, float v) { *p = __float2half_rn(v); }
-template <> __device__ __forceinline__ void put<__nv_bfloat16>(__nv_bfloat16 *p, float v) {
-    *p = __float2bfloat16_rn(v);
-}
-
-// Eight query elements as fp16 words, b[0..3] = pairs (e, e + 4): the order
-// in which unpack_int() leaves a word's codes.
-template <typename T>
-__device__ __forceinline__ void load_q8(const T *p, bool vec, float (&v)[8]) {
-    alignas(16) T e[8];
-    if (vec) {
-        *reinterpret_cast<uint4 *>(e) = __ldg(reinterpret_cast<const uint4 *>(p));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f32(e[i]);
 }
 
 // One CTA = four warps over an equal share of all rounds (64 tokens of one
@@ -307,17 +258,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                     top = fmaxf(top, fabsf(v[c][e]));
                 }
             }
-            float up = 1.0f, down = 1.0f;  // q * up in fp16, scores * down
             if (!std::is_same<T, __half>::value) {
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int ex = (int)(__float_as_uint(top) >> 23);  // biased; 0: zero or subnormal, 255: inf
-                if (ex > 0 && ex < 255) {
-                    const int sh = min(135 - ex, 100);  // largest element to [2^8, 2^9)
-                    up = __uint_as_float((uint32_t)(127 + sh) << 23);
-                    down = __uint_as_float((uint32_t)(127 - sh) << 23);
-                }
             }
+            float down;  // q * up in fp16, scores * down
+            const float up = fp16_power<T>(top, down);
 #pragma unroll
             for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -657,6 +603,10 @@ constexpr size_t ring_bytes() {
 
 size_t header_bytes(const oq_kv4_batch *b) { return (size_t)cdiv((b->sequences + 1) * 8, 128) * 128; }
 
+// Sequences of up to kFew query rows a key head are streamed, the others go to
+// the prompt kernel.
+constexpr int kFew = 32;
+
 int columns_of(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
     return (int64_t)b->max_tokens * (q_heads / c->kv_heads) <= 8 ? 1 : 2;
 }
@@ -676,8 +626,9 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
     kern<<<share, kWarps * 32, smem, st>>>(a);
     if (int rc = check_launch("kv4_attention")) return rc;
 
-    const int64_t blocks = cdiv((int64_t)batch->max_tokens * a.ratio, 8 * NT), items = blocks * a.kv_heads;
-    OQ_REQUIRE(items <= 65535, "kv4_attention: too many query rows per sequence");
+    const int64_t most = (int64_t)batch->max_tokens * a.ratio;
+    const int64_t blocks = cdiv(most < a.few ? most : a.few, 8 * NT), items = blocks * a.kv_heads;
+    OQ_REQUIRE(items <= 65535, "kv4_attention: too many key heads");
     const bool split = (int64_t)share > 16 * items * batch->sequences;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(split ? 8 * NT : 1, (unsigned)items, batch->sequences);
@@ -773,6 +724,13 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     a.vec = aligned(q, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const int nt = columns_of(cache, batch, q_heads);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t most = (int64_t)batch->max_tokens * a.ratio;  // rows a sequence and key head
+    a.few = a.ratio > kFew ? a.ratio : kFew;                   // single tokens are always streamed
+    if (most > a.few) {
+        // sum over sequences of ceil(rows / kPromptRows), at most
+        const int64_t items = (cdiv(tokens * a.ratio, kPromptRows) + batch->sequences) * a.kv_heads;
+        if (int rc = prompt_attention(a, dtype, cache, batch->sequences, items, st)) return rc;
+    }
     return dtype == OQ_F16 ? attention_typed<__half>(a, cache, batch, nt, st)
                            : attention_typed<__nv_bfloat16>(a, cache, batch, nt, st);
 }

@@ -1,0 +1,484 @@
+// Attention over the 4-bit key/value cache, many query rows per key head
+// (chunks of prompts): both products on the tcgen05 tensor cores.
+//
+// Mathematics.  A CTA has 256 query rows of one key head -- rows are (token,
+// query head of the key head) in that order, so all query heads that share a
+// key head share its dequantization -- as two tiles of 128, and walks the
+// cache in blocks of 128 tokens:
+//     S = Q K^T (fp32 in TMEM),  p = 2^(S f - m),  O = O + P V
+// with the running maximum m of a row raised only when a score passes it by
+// 2^14 (see kRaise): then O, in TMEM, is multiplied by 2^(m_old - m_new);
+// otherwise it is not touched.  K and V go to shared memory as code * scale,
+// which are fp16 numbers exactly; P is rounded to fp16 (at most 2^14, largest
+// at least 2^6) and goes back into S's TMEM columns as the second product's
+// A operand.  Queries are fp16 (bf16 rows times a power of two).
+//
+// Roles: warps 0-3 and 4-7 are the softmax of the two tiles (a thread a row),
+// warps 8-11 turn codes into fp16 tiles, one thread of warp 12 issues the
+// products.  While one tile's softmax runs, the other tile's products do:
+// the issue order is P0 V, Q0 K', P1 V, Q1 K', ...
+//
+// Layouts: Q and K tiles are K-major, 128-byte swizzled, 64 elements a panel;
+// V tiles have the same bytes (row = token) read as an MN-major operand.
+// Within each eight elements of head_dim the order is that in which
+// unpack_int() leaves a word's codes (0 4 1 5 2 6 3 7): the same for Q and K,
+// and undone for V in the epilogue.
+#include "oq_kv4_attention.cuh"
+
+namespace oq {
+namespace kv4 {
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kTok = 128;  // cached tokens of a block
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kS = 0, kO = 256;  // TMEM columns: S tiles at 0 and 128, O tiles at 256 and 256 + head_dim
+constexpr int kSoftmaxRegs = 184, kDequantRegs = 104, kIssueRegs = 40;
+static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * (65536 / kThreads), "register split");
+
+template <int HD>
+struct Smem {
+    static constexpr int kPanel = kTok * 128;          // 64 elements of 128 rows
+    static constexpr int kTile = kPanel * (HD / 64);   // Q, K or V tile
+    static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kBars = 6 * kTile;
+    static constexpr int kBytes = kBars + 256 + 1024;  // barriers; slack to align to 1024
+};
+
+// tcgen05.mma B operand, MN-major, 128-byte swizzle: rows (k) of 64 elements,
+// 8-row groups 1024 B apart, panels of 64 elements (mn) `panel` bytes apart.
+__device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, int panel) {
+    return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
+           (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+template <int R>
+__device__ __forceinline__ void regs_inc() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(R));
+}
+template <int R>
+__device__ __forceinline__ void regs_dec() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
+}
+
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// Byte offset of the 16-byte chunk `c` (eight elements) of row r.
+template <int HD>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return (uint32_t)((c >> 3) * Smem<HD>::kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+template <typename T, int HD, int GS>
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a) {
+    using L = Smem<HD>;
+    constexpr int NG = HD / GS, CH = HD / 32;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
+    uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
+    uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *k_full = bars + 6, *k_empty = bars + 8,
+             *v_full = bars + 10, *v_empty = bars + 12, *done = bars + 14;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- this CTA's item: items before each sequence, then the sequence
+    __shared__ int warp_sum[kThreads / 32], found[2];
+    {
+        int base = 0;
+        if (tid == 0) found[0] = -1;
+        __syncthreads();
+        for (int b0 = 0; b0 < a.batch.sequences; b0 += kThreads) {
+            const int b = b0 + tid;
+            int n = 0;
+            if (b < a.batch.sequences) {
+                int first, count;
+                tokens_of(a.batch, b, a.tokens, first, count);
+                const int64_t rows = (int64_t)count * a.ratio;
+                if (rows > a.few) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
+            }
+            int inc = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= o) inc += v;
+            }
+            if (lane == 31) warp_sum[warp] = inc;
+            __syncthreads();
+            int before = base;
+            for (int w = 0; w < kThreads / 32; ++w) {
+                if (w < warp) before += warp_sum[w];
+                base += warp_sum[w];
+            }
+            before += inc - n;
+            if ((int)blockIdx.x >= before && (int)blockIdx.x < before + n) {
+                found[0] = b;
+                found[1] = blockIdx.x - before;
+            }
+            __syncthreads();
+        }
+    }
+    const int b = found[0];
+    if (b < 0) return;
+    int first, count;
+    tokens_of(a.batch, b, a.tokens, first, count);
+    const int length = length_of(a.batch, b, a.page_size);
+    const int rows = count * a.ratio, blocks = (rows + kPromptRows - 1) / kPromptRows;
+    // the last rows see most: they go first
+    const int head = found[1] % a.kv_heads, row0 = (blocks - 1 - found[1] / a.kv_heads) * kPromptRows;
+    const int nrows = min(kPromptRows, rows - row0);
+    const int64_t base = (int64_t)length - count;  // position of the step's first token
+    const int64_t p0 = base + row0 / a.ratio, p1 = base + (row0 + nrows - 1) / a.ratio;
+    const int64_t hi = a.causal ? p1 + 1 : length;
+    const int64_t floor = a.window > 0 ? max(p0 + 1 - a.window, (int64_t)0) : 0;
+    const int64_t lo = floor & ~15ll;
+    const int nblk = hi > lo ? (int)((hi - lo + kTok - 1) / kTok) : 0;
+    const int tiles = nrows > 128 ? 2 : 1;
+
+    if (tid == 0) {
+        mbar_init(&q_full[0], 128 * tiles);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128);
+            mbar_init(&k_full[i], 128);
+            mbar_init(&v_full[i], 128);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+        }
+        mbar_init(done, 1);
+        fence_barrier_init();
+    }
+    if (warp == 12) {
+        tmem_alloc(tmem_slot, kTmemCols);
+        tmem_relinquish();
+        tc_fence_before();
+    }
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    if (warp < 8) {
+        // -------------------------------------------------------- softmax
+        regs_inc<kSoftmaxRegs>();
+        const int wg = warp >> 2, r = tid & 127;
+        const int row = row0 + wg * 128 + r;
+        const bool in = row < rows;
+        if (wg < tiles) {
+            const int tk = in ? row / a.ratio : 0;
+            const int64_t at = (int64_t)(first + tk) * a.q_heads + head * a.ratio + (in ? row - tk * a.ratio : 0);
+            float f = fabsf(a.f);
+            {
+                const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tk) * a.q_ts +
+                               (int64_t)(head * a.ratio + (in ? row - tk * a.ratio : 0)) * a.q_hs;
+                float top = 0.0f, v[8], down;
+                if (!std::is_same<T, __half>::value && in) {
+                    for (int c = 0; c < HD / 8; ++c) {
+                        load_q8<T>(src + 8 * c, a.vec, v);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+                    }
+                }
+                float up = fp16_power<T>(top, down);
+                f *= down;
+                if (a.f < 0.0f) up = -up;
+                const uint32_t dst = smem_u32(smem + L::kQ + wg * L::kTile);
+                for (int c = 0; c < HD / 8; ++c) {
+                    uint32_t w[4] = {0, 0, 0, 0};
+                    if (in) {
+                        load_q8<T>(src + 8 * c, a.vec, v);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up));
+                    }
+                    st16(dst + chunk_at<HD>(r, c), w[0], w[1], w[2], w[3]);
+                }
+                fence_async_smem();
+                mbar_arrive(&q_full[0]);
+            }
+            if (f == 0.0f) f = 1e-30f;  // masked scores are -inf before they are multiplied
+            const int64_t pos = base + tk;
+            const int64_t vis = a.causal ? pos + 1 : length, low = a.window > 0 ? pos + 1 - a.window : 0;
+            // tokens that every row of the tile sees
+            const int last = min(row0 + wg * 128 + 127, rows - 1);
+            const int64_t all_vis = a.causal ? base + (row0 + wg * 128) / a.ratio + 1 : length;
+            const int64_t all_low = a.window > 0 ? base + last / a.ratio + 1 - a.window : 0;
+            const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
+            const uint32_t ts = tmem + quarter + kS + wg * 128, to = tmem + quarter + kO + wg * HD;
+            float m = -1e30f, l = 0.0f;
+            bool ok = true;
+            for (int j = 0; j < nblk; ++j) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[wg], j & 1));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t s[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) tmem_ld_32x32b_x32(ts + 32 * i, s[i]);
+                tc_wait_ld();
+                const int64_t t0 = lo + (int64_t)j * kTok;
+                if (t0 + kTok > all_vis || t0 < all_low) {
+                    const int e0 = (int)min(max(low - t0, (int64_t)0), (int64_t)kTok);
+                    const int e1 = (int)min(max(vis - t0, (int64_t)0), (int64_t)kTok);
+#pragma unroll
+                    for (int i = 0; i < 128; ++i)
+                        if (i < e0 || i >= e1) s[i >> 5][i & 31] = 0xff800000u;
+                }
+                float mx[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    mx[i] = __uint_as_float(s[i][0]);
+#pragma unroll
+                    for (int e = 1; e < 32; ++e) mx[i] = fmaxf(mx[i], __uint_as_float(s[i][e]));
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
+                const bool raise = top > m + kRaise;
+                if (__any_sync(0xffffffffu, raise)) {
+                    const float mn = raise ? top - kLift : m, corr = ex2(m - mn);
+                    l *= corr;
+                    m = mn;
+                    if (j > 0) {  // P V of the block before is complete: it was issued before this S
+#pragma unroll
+                        for (int i = 0; i < HD / 32; ++i) {
+                            uint32_t o[32];
+                            tmem_ld_32x32b_x32(to + 32 * i, o);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                            tmem_st_32x32b_x32(to + 32 * i, o);
+                        }
+                    }
+                }
+                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int c = 64 * i + 2 * e;
+                        const float x = ex2(fmaf(__uint_as_float(s[c >> 5][c & 31]), f, -m));
+                        const float y = ex2(fmaf(__uint_as_float(s[(c + 1) >> 5][(c + 1) & 31]), f, -m));
+                        sum[e & 1] += x;
+                        sum[2 + (e & 1)] += y;
+                        p[e] = as_u32(__floats2half2_rn(x, y));
+                    }
+                    tmem_st_32x32b_x32(ts + 32 * i, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                tc_wait_st();
+                tc_fence_before();
+                mbar_arrive(&p_full[wg]);
+            }
+            // ------------------------------------------------- epilogue
+            if (nblk > 0) {
+                ok = __all_sync(0xffffffffu, ok && mbar_wait(done, 0));
+                tc_fence_after();
+            }
+            if (ok) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+                T *dst = static_cast<T *>(a.out) + at * HD;
+#pragma unroll
+                for (int i = 0; i < HD / 32; ++i) {
+                    uint32_t o[32];
+                    if (nblk > 0) {
+                        tmem_ld_32x32b_x32(to + 32 * i, o);
+                        tc_wait_ld();
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0;
+                    }
+                    if (in) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            alignas(16) T v[8];
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)  // column e holds element 0 4 1 5 2 6 3 7
+                                put(&v[(e >> 1) + (e & 1) * 4], __uint_as_float(o[8 * c + e]) * inv);
+                            reinterpret_cast<uint4 *>(dst + 32 * i)[c] = *reinterpret_cast<uint4 *>(v);
+                        }
+                    }
+                }
+                if (in && a.log_sum != nullptr)
+                    a.log_sum[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+            }
+        }
+    } else if (warp < 12) {
+        // ---------------------------------------------------- dequantize
+        regs_dec<kDequantRegs>();
+        constexpr int N = HD / 32;  // 16-byte chunks of codes a thread takes of a K or V block
+        const int r = tid & 127;
+        const int per = a.page_size >> 4;
+        uint32_t row16 = 0;  // lane i < 8: row / 16 in the cache of the block's i-th 16 tokens
+        auto look_up = [&](int j) {
+            uint32_t v = 0;
+            const int64_t t = lo + (int64_t)j * kTok + lane * 16;
+            if (lane < 8 && t < hi && t + 16 > floor) {
+                const int blk = (int)(t >> 4), pg = blk / per;
+                const int page = __ldg(a.batch.table + (int64_t)b * a.batch.max_pages + pg);
+                if (page < 0 || page >= a.pages)
+                    index_error();
+                else
+                    v = (uint32_t)(((int64_t)page * a.kv_heads + head) * per + (blk - pg * per));
+            }
+            return v;
+        };
+        uint4 kc[N], vc[N];
+        uint32_t sc[N];  // scales of a chunk: K low, V high half
+        // chunk i of the thread: token (r + 128 i) / CH, 16-byte chunk (r + 128 i) % CH
+        auto load = [&](int j, bool keys) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int id = r + 128 * i, tk = id / CH, c = id % CH;
+                const uint32_t r16 = __shfl_sync(0xffffffffu, row16, tk >> 4);
+                const size_t row = (size_t)r16 * 16 + (tk & 15);
+                const int64_t t = lo + (int64_t)j * kTok + tk;
+                // tokens that no row of the block sees may be anything: they become 0
+                const bool live = t < hi && t >= floor;
+                const uint8_t *codes = (keys ? a.k_codes : a.v_codes) + row * (HD / 2) + c * 16;
+                const __half *scale = (keys ? a.k_scales : a.v_scales) + row * NG + c * 32 / GS;
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(codes));
+                const uint32_t s = live ? (uint32_t)__half_as_ushort(__ldg(scale)) : 0u;
+                if (keys) {
+                    kc[i] = w;
+                    sc[i] = (sc[i] & 0xffff0000u) | s;
+                } else {
+                    vc[i] = w;
+                    sc[i] = (sc[i] & 0xffffu) | s << 16;
+                }
+            }
+        };
+        auto store = [&](uint32_t dst, const uint4 (&w)[N], bool keys) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int id = r + 128 * i, tk = id / CH, c = id % CH;
+                const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)(keys ? sc[i] & 0xffffu : sc[i] >> 16)));
+                uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
+                // the upper chunks of a row take their words in the order 2 3 0 1:
+                // the eight lanes of a 128-byte store then hit different banks
+                const bool swap = CH == 4 && (c & 2);
+                if (swap) {
+                    uint32_t t = word[0];
+                    word[0] = word[2], word[2] = t;
+                    t = word[1];
+                    word[1] = word[3], word[3] = t;
+                }
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    __half2 v[4];
+                    unpack_int(word[x], v);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = __hmul2(v[e], s2);
+                    st16(dst + chunk_at<HD>(tk, 4 * c + (x ^ (swap ? 2 : 0))), as_u32(v[0]), as_u32(v[1]), as_u32(v[2]),
+                         as_u32(v[3]));
+                }
+            }
+        };
+        if (nblk > 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sc[i] = 0;
+            row16 = look_up(0);
+            load(0, true);
+            load(0, false);
+            row16 = look_up(1);
+        }
+        bool ok = true;
+        for (int j = 0; j < nblk; ++j) {
+            const int st = j & 1;
+            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((j >> 1) - 1) & 1));
+            if (!ok) break;
+            store(smem_u32(smem + L::kK + st * L::kTile), kc, true);
+            fence_async_smem();
+            mbar_arrive(&k_full[st]);
+            if (j + 1 < nblk) load(j + 1, true);
+            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((j >> 1) - 1) & 1));
+            if (!ok) break;
+            store(smem_u32(smem + L::kV + st * L::kTile), vc, false);
+            fence_async_smem();
+            mbar_arrive(&v_full[st]);
+            if (j + 1 < nblk) load(j + 1, false);
+            row16 = look_up(j + 2);
+        }
+    } else {
+        // --------------------------------------------------------- issue
+        regs_dec<kIssueRegs>();
+        if (warp == 12 && lane == 0 && nblk > 0) {
+            constexpr uint32_t id_qk = umma_idesc_f16(128, kTok, false);
+            constexpr uint32_t id_pv = umma_idesc_f16(128, HD, false) | 1u << 16;  // B is MN-major
+            const uint32_t q0 = smem_u32(smem + L::kQ);
+            auto scores = [&](int i, int j) {
+                const uint64_t qd = umma_desc_sw128(q0 + i * L::kTile);
+                const uint64_t kd = umma_desc_sw128(smem_u32(smem + L::kK + (j & 1) * L::kTile));
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) {
+                    const uint64_t off = (uint64_t)((k >> 2) * L::kPanel + (k & 3) * 32) >> 4;
+                    tc_mma_ss(tmem + kS + i * 128, qd + off, kd + off, id_qk, k != 0);
+                }
+                tc_commit(&s_full[i]);
+            };
+            auto values = [&](int i, int j) {
+                const uint64_t vd = desc_mn_sw128(smem_u32(smem + L::kV + (j & 1) * L::kTile), L::kPanel);
+#pragma unroll
+                for (int k = 0; k < kTok / 16; ++k)
+                    tc_mma_ts(tmem + kO + i * HD, tmem + kS + i * 128 + k * 8, vd + (uint64_t)(k * 16 * 128 >> 4),
+                              id_pv, j != 0 || k != 0);
+            };
+            bool ok = mbar_wait(&q_full[0], 0) && mbar_wait(&k_full[0], 0);
+            if (ok) {
+                tc_fence_after();
+                for (int i = 0; i < tiles; ++i) scores(i, 0);
+                tc_commit(&k_empty[0]);
+            }
+            for (int j = 0; ok && j < nblk; ++j) {
+                if (!(ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1))) break;
+                for (int i = 0; i < tiles; ++i) {
+                    if (!(ok = mbar_wait(&p_full[i], j & 1))) break;
+                    tc_fence_after();
+                    values(i, j);
+                    if (i == tiles - 1) tc_commit(&v_empty[j & 1]);
+                    if (j + 1 < nblk) {
+                        if (i == 0 && !(ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1))) break;
+                        tc_fence_after();
+                        scores(i, j + 1);
+                        if (i == tiles - 1) tc_commit(&k_empty[(j + 1) & 1]);
+                    }
+                }
+            }
+            // Every product this thread issued has completed once `done` fires.
+            tc_commit(done);
+            mbar_wait(done, 0);
+        }
+        __syncwarp();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 12) tmem_dealloc(tmem, kTmemCols);
+}
+
+template <typename T, int HD, int GS>
+int launch(const AttnArgs &a, int64_t items, cudaStream_t st) {
+    auto kern = prompt_kernel<T, HD, GS>;
+    if (int rc = allow_dynamic_smem(reinterpret_cast<const void *>(kern), Smem<HD>::kBytes)) return rc;
+    kern<<<(unsigned)items, kThreads, Smem<HD>::kBytes, st>>>(a);
+    return check_launch("kv4_attention (prompt)");
+}
+
+template <typename T>
+int launch_typed(const AttnArgs &a, const oq_kv4_cache *c, int64_t items, cudaStream_t st) {
+    if (c->head_dim == 64)
+        return c->group_size == 32 ? launch<T, 64, 32>(a, items, st) : launch<T, 64, 64>(a, items, st);
+    return c->group_size == 32   ? launch<T, 128, 32>(a, items, st)
+           : c->group_size == 64 ? launch<T, 128, 64>(a, items, st)
+                                 : launch<T, 128, 128>(a, items, st);
+}
+
+}  // namespace
+
+int prompt_attention(const AttnArgs &a, int dtype, const oq_kv4_cache *c, int sequences, int64_t items,
+                     cudaStream_t st) {
+    (void)sequences;
+    OQ_REQUIRE(items < (1ll << 31), "kv4_attention: too many query rows");
+    return dtype == OQ_F16 ? launch_typed<__half>(a, c, items, st) : launch_typed<__nv_bfloat16>(a, c, items, st);
+}
+
+}  // namespace kv4
+}  // namespace oq

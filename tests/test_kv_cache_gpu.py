@@ -440,7 +440,7 @@ def test_attention_scores_far_apart(count):
     case = Case([400], [count], 1, 64, page=16)
     codes, scales = case.arrays[0]
     for j in range(400):
-        scales[case.table[0, j // 16], 0, j % 16] = np.float16((j + 1) / 32)
+        scales[case.table[0, j // 16], 0, j % 16] = ko.bf16((j + 1) / 32)  # 8 significant bits, as the format has
     case.cache.k_scales.copy_(torch.from_numpy(scales))
     for size, dtype in ((3.0, torch.float16), (1e-3, torch.float16), (300.0, torch.bfloat16), (1e-30, torch.bfloat16)):
         q = case.queries(3, 64, dtype, size=size)
