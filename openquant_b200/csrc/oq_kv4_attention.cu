@@ -22,27 +22,29 @@ namespace oq {
 namespace kv4 {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kTile = 16 * kWarps;  // cached tokens of one round of a CTA
-constexpr int kStages = 4;          // 16-token stages a warp has in flight or in use
+constexpr int kWarps = 4;   // warps a CTA; each works by itself
+constexpr int kStages = 4;  // 16-token stages of a warp: a pair in use, a pair in flight
+constexpr int kSetup = 6;   // cost of beginning an item, in blocks of 16 tokens
+constexpr int kLeast = 10;  // smallest share of a warp, in the same unit
 
 using Args = AttnArgs;
 
-// Columns (query rows) of a partial, and its floats: m[cols], l[cols], o[cols][HD].
+// A partial result: m[cols], l[cols], then o as the lanes hold it (float4
+// [NT * HD / 16][32 lanes]: coalesced, and the joining kernel has the same lanes).
 template <int HD, int NT>
 struct Shape {
     static constexpr int kCols = 8 * NT;
-    static constexpr int kPart = kCols * (HD + 2);
+    static constexpr int kSlices = NT * HD / 16;
+    static constexpr int kPart = 2 * kCols + kSlices * 128;
     static constexpr int kPitch = HD / 2 + 16;  // bytes of a staged row: 16-byte steps over all banks
 };
 
-// Work of sequence b: `tiles` rounds per item, an item per key head and per
-// block of kCols query rows.
+// Work of sequence b: an item per key head and per block of `cols` query
+// rows, of nb blocks of 16 cached tokens (from block b0 on) and kSetup units.
 struct Work {
     int first, count, rows, length;
-    int64_t floor;  // first cached token any row sees
-    int64_t lo;     // the same down to a tile
-    int tiles, blocks;
+    int floor;  // first cached token any row sees
+    int b0, nb, blocks;
 };
 
 __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
@@ -51,12 +53,16 @@ __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
     w.length = length_of(a.batch, b, a.page_size);
     w.rows = w.count * a.ratio;
     w.blocks = w.rows > a.few ? 0 : (w.rows + cols - 1) / cols;
-    w.floor = 0;
-    if (a.window > 0) w.floor = max((int64_t)w.length - w.count + 1 - a.window, (int64_t)0);
-    w.lo = w.floor / kTile * kTile;
-    const int64_t n = ((int64_t)w.length - w.lo + kTile - 1) / kTile;
-    w.tiles = n > 1 ? (int)n : 1;
+    w.floor = a.window > 0 ? (int)max((int64_t)w.length - w.count + 1 - a.window, (int64_t)0) : 0;
+    w.b0 = w.floor >> 4;
+    w.nb = max(((w.length + 15) >> 4) - w.b0, 1);
     return w;
+}
+
+// Warps that share `all` units.
+__device__ __forceinline__ int64_t shares_of(int64_t all, int warps) {
+    const int64_t n = (all + kLeast - 1) / kLeast;
+    return n < warps ? (n > 0 ? n : 1) : warps;
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
@@ -67,13 +73,13 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t d;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
     return d;
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -88,13 +94,28 @@ __device__ __forceinline__ void cp_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// One CTA = four warps over an equal share of all rounds (64 tokens of one
-// item), so that ragged lengths load every SM alike: a share begins and ends
-// inside an item, whose parts the joining kernel adds in a fixed order.  A
-// warp streams its own 16 tokens of each round through a ring of cp.async
-// stages; the rows are staged 16 bytes longer than they are, which makes both
-// the ldmatrix of the keys and the 4- or 8-byte reads of the values free of
-// bank conflicts.
+// Writes a warp's columns of an item: sums reduced over the lanes already, o
+// divided by them.
+template <typename T, int HD>
+__device__ __forceinline__ void write_slice(const Args &a, const Work &w, int head, int col, int d, float x, float y,
+                                            float m, float l) {
+    if (col >= w.rows) return;
+    const int tk = col / a.ratio;
+    const int64_t row = (int64_t)(w.first + tk) * a.q_heads + head * a.ratio + (col - tk * a.ratio);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *dst = static_cast<T *>(a.out) + row * HD + d;
+    put(dst, x * inv);
+    put(dst + 1, y * inv);
+    if (d == 0 && a.log_sum != nullptr) a.log_sum[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
+// Every warp takes an equal share of all blocks of all items, one after the
+// other: ragged lengths load the warps alike, and no warp waits for another.
+// A share begins and ends inside an item, whose parts the joining kernel adds
+// in a fixed order.  A warp streams its blocks through its own ring of cp.async
+// stages, two blocks at a time (two independent chains of products); the rows
+// are staged 16 bytes longer than they are, which makes both the ldmatrix of
+// the keys and the 4- or 8-byte reads of the values free of bank conflicts.
 template <typename T, int HD, int GS, int NT>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(const Args a) {
     using S = Shape<HD, NT>;
@@ -108,6 +129,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     unsigned char *ring = smem + warp * kStages * kStage;
     int64_t *prefix = reinterpret_cast<int64_t *>(smem + kWarps * kStages * kStage);
+    asm volatile("griddepcontrol.launch_dependents;");
 
     // ---- units before each sequence (exclusive prefix in shared memory)
     {
@@ -118,7 +140,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             int64_t n = 0;
             if (b < a.batch.sequences) {
                 const Work w = work_of(a, b, kCols);
-                n = (int64_t)w.tiles * w.blocks * a.kv_heads;
+                n = (int64_t)(w.nb + kSetup) * w.blocks * a.kv_heads;
             }
             int64_t inc = n;
 #pragma unroll
@@ -143,8 +165,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         if (blockIdx.x == 0)
             for (int b = tid; b <= a.batch.sequences; b += kWarps * 32) a.prefix[b] = prefix[b];
     }
-    const int64_t all = prefix[a.batch.sequences];
-    const int64_t u0 = (int64_t)blockIdx.x * all / gridDim.x, u1 = ((int64_t)blockIdx.x + 1) * all / gridDim.x;
 
     // Padding tokens: 0, log-sum -inf.
     {
@@ -157,6 +177,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             if (lane == 0 && a.log_sum != nullptr) a.log_sum[row] = -INFINITY;
         }
     }
+
+    const int64_t all = prefix[a.batch.sequences];
+    const int64_t shares = shares_of(all, gridDim.x * kWarps);
+    const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbouring shares on different SMs
+    if (me >= shares) return;
+    const int64_t u0 = me * all / shares, u1 = (me + 1) * all / shares;
 
     for (int64_t u = u0; u < u1;) {
         // ---- the item of unit u
@@ -174,45 +200,35 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         }
         const Work w = work_of(a, b, kCols);
         const int64_t local = u - prefix[b];
-        const int item = (int)(local / w.tiles), tile0 = (int)(local - (int64_t)item * w.tiles);
-        const int tile1 = (int)min((int64_t)w.tiles, tile0 + (u1 - u));
-        const int head = item / w.blocks, row0 = (item - head * w.blocks) * kCols;
-        const bool whole = tile0 == 0 && tile1 == w.tiles;
+        const int per = w.nb + kSetup, item = (int)(local / per), off = (int)(local - (int64_t)item * per);
+        const int take = (int)min((int64_t)(per - off), u1 - u);
+        const int i0 = max(off - kSetup, 0), i1 = off + take - kSetup;  // blocks [i0, i1) of the item
         const int slot = u == u0 ? 0 : 1;  // a part is the share's first item or its last
-        u += tile1 - tile0;
-
-        // ---- this warp's 16-token blocks: tokens tok0 + i * kTile, i < nblk
-        const int64_t tok0 = w.lo + (int64_t)tile0 * kTile + warp * 16;
-        int nblk = tile1 - tile0;
-        {
-            const int64_t left = (int64_t)w.length - tok0;  // tokens from tok0 on
-            const int64_t most = left > 0 ? (left + kTile - 1) / kTile : 0;
-            if (most < nblk) nblk = (int)most;
-        }
+        u += take;
+        if (i1 <= i0) continue;
+        const bool whole = i0 == 0 && i1 == w.nb;
+        const int head = item / w.blocks, row0 = (item - head * w.blocks) * kCols;
+        const int first_tok = (w.b0 + i0) * 16;
+        // blocks of this part; a sequence of length 0 has one without tokens
+        const int nblk = first_tok < w.length ? i1 - i0 : 0;
 
         // Row numbers / 16 in the cache of the next 32 blocks, one a lane.
         uint32_t rows16 = 0;
-        auto look_up = [&](int i0) {
-            const int i = i0 + lane;
+        auto look_up = [&](int n0) {
             rows16 = 0;
-            // blocks below every window are staged (row 0 of the cache) but not looked up:
-            // their pages may be gone
-            if (i < nblk && tok0 + (int64_t)i * kTile + 16 > w.floor) {
-                const int64_t blk = (tok0 + (int64_t)i * kTile) >> 4;
-                const int per = a.page_size >> 4;
-                const int pg = (int)(blk / per);
+            if (n0 + lane < nblk) {
+                const int blk = w.b0 + i0 + n0 + lane, pp = a.page_size >> 4, pg = blk / pp;
                 const int page = __ldg(a.batch.table + (int64_t)b * a.batch.max_pages + pg);
                 if (page < 0 || page >= a.pages)
                     index_error();
                 else
-                    rows16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * per + (blk - (int64_t)pg * per));
+                    rows16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * pp + (blk - pg * pp));
             }
         };
         auto load = [&](int i) {
             if (i < nblk) {
                 const uint32_t r16 = __shfl_sync(0xffffffffu, rows16, i & 31);
-                unsigned char *st = ring + (i % kStages) * kStage;
-                const uint32_t dst = smem_u32(st);
+                const uint32_t dst = smem_u32(ring) + (i % kStages) * kStage;
                 const uint8_t *ks = a.k_codes + (size_t)r16 * (16 * HD / 2);
                 const uint8_t *vs = a.v_codes + (size_t)r16 * (16 * HD / 2);
 #pragma unroll
@@ -222,24 +238,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                     cp16(to, ks + ch * 16);
                     cp16(to + kCodes, vs + ch * 16);
                 }
-                if (lane < 2 * NG)
-                    cp16(dst + 2 * kCodes + lane * 16,
-                         reinterpret_cast<const unsigned char *>(a.k_scales) + (size_t)r16 * kScales + lane * 16);
-                else if (lane < 4 * NG)
-                    cp16(dst + 2 * kCodes + lane * 16, reinterpret_cast<const unsigned char *>(a.v_scales) +
-                                                           (size_t)r16 * kScales + (lane - 2 * NG) * 16);
+                if (lane < 4 * NG) {
+                    const unsigned char *sc = reinterpret_cast<const unsigned char *>(lane < 2 * NG ? a.k_scales
+                                                                                                    : a.v_scales);
+                    cp16(dst + 2 * kCodes + lane * 16, sc + (size_t)r16 * kScales + (lane % (2 * NG)) * 16);
+                }
             }
-            cp_commit();
         };
         look_up(0);
-#pragma unroll
-        for (int i = 0; i < kStages - 1; ++i) load(i);
+        __syncwarp();  // the ring's last reads (of the item before) are done
+        load(0);
+        load(1);
+        cp_commit();
+        load(2);
+        load(3);
+        cp_commit();
 
         // ---- queries: column n = 8 j + g of this lane as B fragments
         uint32_t qf[NT][CH][4];
-        float f[NT][2];              // factor of columns 8 j + 2 t4 and + 1
-        int64_t vis[NT][2], low[NT][2];  // their visible tokens [low, vis)
-        int64_t all_vis = w.length, all_low = 0;  // visible to every column
+        float f[NT][2];            // factor of columns 8 j + 2 t4 and + 1
+        int vis[NT][2], low[NT][2];  // their visible tokens [low, vis)
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int n = row0 + 8 * j + g;
@@ -247,49 +265,49 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             const int tk = in ? n / a.ratio : 0;
             const T *src = static_cast<const T *>(a.q) + (int64_t)(w.first + tk) * a.q_ts +
                            (int64_t)(head * a.ratio + (in ? n - tk * a.ratio : 0)) * a.q_hs;
-            float top = 0.0f;
-            float v[CH][8];
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                if (in) load_q8<T>(src + 32 * c + 8 * t4, a.vec, v[c]);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    if (!in) v[c][e] = 0.0f;
-                    top = fmaxf(top, fabsf(v[c][e]));
-                }
-            }
+            float top = 0.0f, v[8];
             if (!std::is_same<T, __half>::value) {
+                if (in) {
+#pragma unroll
+                    for (int c = 0; c < CH; ++c) {
+                        load_q8<T>(src + 32 * c + 8 * t4, a.vec, v);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+                    }
+                }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             }
             float down;  // q * up in fp16, scores * down
-            const float up = fp16_power<T>(top, down);
+            float up = fp16_power<T>(top, down);
+            if (a.f < 0.0f) up = -up;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+            for (int c = 0; c < CH; ++c) {
+                if (in) load_q8<T>(src + 32 * c + 8 * t4, a.vec, v);
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
-                    qf[j][c][e] = as_u32(__floats2half2_rn(v[c][e] * up, v[c][e + 4] * up));
-            const float fn = a.f * down;
+                    qf[j][c][e] = in ? as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up)) : 0u;
+            }
+            const float fn = fmaxf(fabsf(a.f) * down, 1e-30f);  // not 0: masked scores are -inf before the product
             f[j][0] = __shfl_sync(0xffffffffu, fn, 8 * t4);
             f[j][1] = __shfl_sync(0xffffffffu, fn, 8 * t4 + 4);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = row0 + 8 * j + 2 * t4 + e;
-                const int64_t p = (int64_t)w.length - w.count + (col < w.rows ? col / a.ratio : w.count - 1);
+                const int p = w.length - w.count + (col < w.rows ? col / a.ratio : w.count - 1);
                 vis[j][e] = a.causal ? p + 1 : w.length;
-                low[j][e] = a.window > 0 ? p + 1 - a.window : 0;
+                low[j][e] = a.window > 0 ? (int)max((int64_t)p + 1 - a.window, (int64_t)0) : 0;
             }
         }
-        {
-            const int64_t p0 = (int64_t)w.length - w.count + row0 / a.ratio;  // the first row's position
-            if (a.causal) all_vis = p0 + 1;
-            if (a.window > 0) {
-                const int last = min(row0 + kCols, w.rows) - 1;
-                all_low = (int64_t)w.length - w.count + last / a.ratio + 1 - a.window;
-            }
+        // tokens that every column of the item sees
+        int all_vis = w.length, all_low = 0;
+        if (a.causal) all_vis = w.length - w.count + row0 / a.ratio + 1;
+        if (a.window > 0) {
+            const int last = min(row0 + kCols, w.rows) - 1;
+            all_low = (int)max((int64_t)w.length - w.count + last / a.ratio + 1 - a.window, (int64_t)0);
         }
 
-        float o[NT][HD / 16][4], m[NT][2], l[NT][2];
+        float o[NT][HD / 16][4], m[NT][2], l[NT][2], most[NT][2];  // most: the score at which m is raised
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -297,27 +315,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][i][e] = 0.0f;
             m[j][0] = m[j][1] = -1e30f;
+            most[j][0] = most[j][1] = -INFINITY;
             l[j][0] = l[j][1] = 0.0f;
         }
 
-        for (int i = 0; i < nblk; ++i) {
-            // stage i + kStages - 1 takes the place of stage i - 1, whose reads
-            // ended before the warp's last __syncwarp
-            if (((i + kStages - 1) & 31) == 0) look_up(i + kStages - 1);
-            load(i + kStages - 1);
-            cp_wait<kStages - 1>();
+        for (int i = 0; i < nblk; i += 2) {
+            cp_wait<1>();
             __syncwarp();
-            const unsigned char *st = ring + (i % kStages) * kStage;
-            const uint32_t su = smem_u32(st);
-            const int64_t tok = tok0 + (int64_t)i * kTile;
+            const int tok = first_tok + i * 16;
 
-            // ---- scores of tokens g and g + 8
-            float s[NT][4];
+            // ---- scores of tokens g and g + 8 of both blocks
+            float s[2][NT][4];
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int h = 0; h < 2; ++h) {
+                const unsigned char *st = ring + ((i + h) % kStages) * kStage;
+                const uint32_t su = smem_u32(st);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[j][e] = 0.0f;
-            {
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[h][j][e] = 0.0f;
                 uint32_t kw[2][CH];  // words t4 of each chunk of rows g, g + 8
                 if (CH == 4) {
                     // matrix i of the four: chunk i of rows 0..7
@@ -339,7 +355,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                         kw[1][c] = r[2 + (c & 1)];
                     }
                 }
-                const __half *ksc = reinterpret_cast<const __half *>(st + 2 * kCodes);
+                alignas(8) __half ks[2][NG];
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const unsigned char *p = st + 2 * kCodes + (g + 8 * x) * NG * 2;
+                    if (NG == 4)
+                        *reinterpret_cast<uint2 *>(ks[x]) = *reinterpret_cast<const uint2 *>(p);
+                    else if (NG == 2)
+                        *reinterpret_cast<uint32_t *>(ks[x]) = *reinterpret_cast<const uint32_t *>(p);
+                    else
+                        ks[x][0] = *reinterpret_cast<const __half *>(p);
+                }
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
                     float acc[NT][4];
@@ -361,44 +387,51 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                                      qf[j][c][3]);
                         }
                     }
-                    const float s0 = __half2float(ksc[g * NG + G]), s1 = __half2float(ksc[(g + 8) * NG + G]);
+                    const float s0 = __half2float(ks[0][G]), s1 = __half2float(ks[1][G]);
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        s[j][0] += s0 * acc[j][0];
-                        s[j][1] += s0 * acc[j][1];
-                        s[j][2] += s1 * acc[j][2];
-                        s[j][3] += s1 * acc[j][3];
+                        s[h][j][0] = fmaf(s0, acc[j][0], s[h][j][0]);
+                        s[h][j][1] = fmaf(s0, acc[j][1], s[h][j][1]);
+                        s[h][j][2] = fmaf(s1, acc[j][2], s[h][j][2]);
+                        s[h][j][3] = fmaf(s1, acc[j][3], s[h][j][3]);
                     }
                 }
             }
 
             // ---- weights p = 2^(s f - m)
-            const bool edge = tok + 16 > all_vis || tok < all_low;  // warp-uniform: some column misses some token
+            // some column misses some token of the pair, or the pair is half a one
+            const bool edge = tok + 32 > all_vis || tok < all_low || i + 1 == nblk;
+            if (edge) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int tk = tok + 16 * h + g + (e >> 1) * 8;
+                            if (tk >= vis[j][e & 1] || tk < low[j][e & 1] || i + h >= nblk) s[h][j][e] = -INFINITY;
+                        }
+            }
             bool raise = false;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float x = s[j][e] * f[j][e & 1];
-                    if (edge) {
-                        const int64_t tk = tok + g + (e >> 1) * 8;
-                        if (tk >= vis[j][e & 1] || tk < low[j][e & 1]) x = -INFINITY;
-                    }
-                    s[j][e] = x;
-                    raise |= x > m[j][e & 1] + kRaise;
-                }
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) raise |= s[h][j][e] > most[j][e & 1];
             if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(s[j][e], s[j][e + 2]);
+                        float mx = fmaxf(fmaxf(s[0][j][e], s[0][j][e + 2]), fmaxf(s[1][j][e], s[1][j][e + 2]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m[j][e], mx - kLift);
+                        const float mn = fmaxf(m[j][e], mx * f[j][e] - kLift);
                         const float corr = ex2(m[j][e] - mn);
                         m[j][e] = mn;
+                        most[j][e] = mn > -1e30f ? __fdividef(mn + kRaise, f[j][e]) : -INFINITY;
                         l[j][e] *= corr;
 #pragma unroll
                         for (int i2 = 0; i2 < HD / 16; ++i2) {
@@ -407,23 +440,26 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                         }
                     }
             }
-            uint32_t pf[NT][2];
+            uint32_t pf[2][NT][2];
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                float p[4];
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    p[e] = ex2(s[j][e] - m[j][e & 1]);
-                    l[j][e & 1] += p[e];
+                for (int j = 0; j < NT; ++j) {
+                    float p[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        p[e] = ex2(fmaf(s[h][j][e], f[j][e & 1], -m[j][e & 1]));
+                        l[j][e & 1] += p[e];
+                    }
+                    pf[h][j][0] = transpose8x8(as_u32(__floats2half2_rn(p[0], p[1])));
+                    pf[h][j][1] = transpose8x8(as_u32(__floats2half2_rn(p[2], p[3])));
                 }
-                pf[j][0] = transpose8x8(as_u32(__floats2half2_rn(p[0], p[1])));
-                pf[j][1] = transpose8x8(as_u32(__floats2half2_rn(p[2], p[3])));
-            }
 
             // ---- o += V^T p: rows d = HD/8 g + ..., tokens 2 t4, +1, +8, +9
-            {
-                const unsigned char *vc = st + kCodes;
-                const __half *vsc = reinterpret_cast<const __half *>(st + 2 * kCodes + kScales);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const unsigned char *vc = ring + ((i + h) % kStages) * kStage + kCodes;
+                const __half *vsc = reinterpret_cast<const __half *>(vc + kCodes + kScales);
                 constexpr int W = HD / 64;  // words a lane takes of a token
                 const int G = NG == 1 ? 0 : (HD / 8 * g) / GS;
                 uint32_t vw[4][W];
@@ -440,8 +476,14 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                         vw[k][0] = src[0];
                     }
                     sc[k] = vsc[r * NG + G];
+                }
+                if (edge) {
                     // tokens that no row sees are whatever the page holds: no NaN from there
-                    if (edge && (tok + r >= w.length || tok + r < w.floor)) sc[k] = __ushort_as_half(0);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int tk = tok + 16 * h + 2 * t4 + (k & 1) + (k >> 1) * 8;
+                        if (tk >= w.length || tk < w.floor || i + h >= nblk) sc[k] = __ushort_as_half(0);
+                    }
                 }
                 const __half2 sa = __halves2half2(sc[0], sc[1]), sb = __halves2half2(sc[2], sc[3]);
 #pragma unroll
@@ -462,133 +504,140 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
                                 mma16816(o[j][4 * x + 2 * hw + k], as_u32(va[2 * k]), as_u32(va[2 * k + 1]),
-                                         as_u32(vb[2 * k]), as_u32(vb[2 * k + 1]), pf[j][0], pf[j][1]);
+                                         as_u32(vb[2 * k]), as_u32(vb[2 * k + 1]), pf[h][j][0], pf[h][j][1]);
                     }
                 }
             }
             __syncwarp();
+            // the next pair but one takes the place of this one
+            if (((i + 4) & 31) == 0) look_up(i + 4);
+            load(i + 4);
+            load(i + 5);
+            cp_commit();
         }
         cp_wait<0>();
-        __syncthreads();
 
-        // ---- join the four warps (the ring is free: every copy has landed)
-        float *wm = reinterpret_cast<float *>(smem), *wl = wm + kWarps * kCols, *wo = wl + kWarps * kCols;
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                float x = l[j][e];
-                x += __shfl_xor_sync(0xffffffffu, x, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                const int col = 8 * j + 2 * t4 + e;
-                if (g == 0) {
-                    wm[warp * kCols + col] = m[j][e];
-                    wl[warp * kCols + col] = x;
-                }
-                float *dst = wo + (size_t)(warp * kCols + col) * HD + HD / 8 * g;
+                l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 4);
+                l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 8);
+                l[j][e] += __shfl_xor_sync(0xffffffffu, l[j][e], 16);
+            }
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int i = 0; i < HD / 16; ++i)
-                    *reinterpret_cast<float2 *>(dst + 2 * i) = make_float2(o[j][i][e], o[j][i][e + 2]);
-            }
-        }
-        __syncthreads();
-        float *part = a.parts + ((int64_t)blockIdx.x * 2 + slot) * S::kPart;
-        for (int x = tid; x < kCols * HD / 4; x += kWarps * 32) {
-            const int col = x / (HD / 4), d = x % (HD / 4) * 4;
-            float mx = wm[col];
 #pragma unroll
-            for (int k = 1; k < kWarps; ++k) mx = fmaxf(mx, wm[k * kCols + col]);
-            float sum = 0.0f;
-            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int e = 0; e < 2; ++e)
+                        write_slice<T, HD>(a, w, head, row0 + 8 * j + 2 * t4 + e, HD / 8 * g + 2 * i, o[j][i][e],
+                                           o[j][i][e + 2], m[j][e], l[j][e]);
+        } else {
+            float *part = a.parts + (me * 2 + slot) * S::kPart;
 #pragma unroll
-            for (int k = 0; k < kWarps; ++k) {
-                const float c = ex2(wm[k * kCols + col] - mx);
-                const float4 ov = *reinterpret_cast<const float4 *>(wo + (size_t)(k * kCols + col) * HD + d);
-                sum += c * wl[k * kCols + col];
-                v.x += c * ov.x, v.y += c * ov.y, v.z += c * ov.z, v.w += c * ov.w;
-            }
-            if (!whole) {
-                if (d == 0) {
-                    part[col] = mx;
-                    part[kCols + col] = sum;
+            for (int j = 0; j < NT; ++j) {
+                if (row0 + 8 * j + 2 * t4 < w.rows) {
+                    if (g == 0) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            part[8 * j + 2 * t4 + e] = m[j][e];
+                            part[kCols + 8 * j + 2 * t4 + e] = l[j][e];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < HD / 16; ++i)
+                        reinterpret_cast<float4 *>(part + 2 * kCols)[(j * (HD / 16) + i) * 32 + lane] =
+                            make_float4(o[j][i][0], o[j][i][1], o[j][i][2], o[j][i][3]);
                 }
-                *reinterpret_cast<float4 *>(part + 2 * kCols + col * HD + d) = v;
-            } else if (row0 + col < w.rows) {
-                const int n = row0 + col, tk = n / a.ratio;
-                const int64_t row = (int64_t)(w.first + tk) * a.q_heads + head * a.ratio + (n - tk * a.ratio);
-                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                T *dst = static_cast<T *>(a.out) + row * HD + d;
-                put(dst, v.x * inv), put(dst + 1, v.y * inv), put(dst + 2, v.z * inv), put(dst + 3, v.w * inv);
-                if (d == 0 && a.log_sum != nullptr)
-                    a.log_sum[row] = sum == 0.0f ? -INFINITY : (mx + log2f(sum)) * 0.6931471805599453f;
             }
         }
-        __syncthreads();
     }
 }
 
-// Adds the parts of the items that more than one CTA worked on, in order.  A
-// CTA of eight warps per item: with SPLIT each of its columns has a CTA of
-// its own whose warps share the parts, else each warp takes whole columns.
+// Adds the parts of the items that more than one warp worked on, in order.  A
+// CTA of eight warps an item; a slice is the float4 a lane holds of one
+// product tile.  SPLIT: a CTA per slice, whose warps share the parts (many
+// parts, few items); else a warp per slice.
 template <typename T, int HD, int NT, bool SPLIT>
-__global__ void __launch_bounds__(256) join_kernel(const Args a, int share) {
+__global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
     using S = Shape<HD, NT>;
-    constexpr int kCols = S::kCols, V = HD / 32;
+    constexpr int kCols = S::kCols;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const Work w = work_of(a, b, kCols);
     const int item = blockIdx.y;
     if (item >= w.blocks * a.kv_heads) return;
-    const int64_t all = a.prefix[a.batch.sequences], s = a.prefix[b] + (int64_t)item * w.tiles, e = s + w.tiles;
-    // the CTA that worked on unit u: the last i with i all / share <= u
-    const int64_t c0 = ((s + 1) * share - 1) / all, c1 = (e * share - 1) / all;
+    const int64_t all = a.prefix[a.batch.sequences], shares = shares_of(all, warps);
+    const int64_t s = a.prefix[b] + (int64_t)item * (w.nb + kSetup), e = s + w.nb + kSetup;
+    // the warp that worked on unit u: the last i with i all / shares <= u
+    const int64_t c0 = ((s + kSetup + 1) * shares - 1) / all, c1 = (e * shares - 1) / all;
     if (c0 == c1) return;
+    // (every warp between them has units, as shares <= all; only the first may start before the item)
     const int head = item / w.blocks, row0 = (item - head * w.blocks) * kCols;
-    __shared__ float sm[8], sl[8], so[8][HD];
-    for (int col = SPLIT ? (int)blockIdx.x : warp; col < kCols; col += SPLIT ? kCols : 8) {
-        if (row0 + col >= w.rows) break;  // rows of a block are in order: the rest are past the end too
-        float m = -1e30f, l = 0.0f, o[V];
+    const float *first = a.parts + (c0 * 2 + (c0 * all / shares >= s ? 0 : 1)) * S::kPart;
+    const float *rest = a.parts + c0 * 2 * S::kPart;  // part n > 0: rest + n * 2 * kPart
+    const int parts = (int)(c1 - c0) + 1;
+    __shared__ float4 so[8][32];
+    __shared__ float sl[8][kCols];
+    for (int sl_i = SPLIT ? (int)blockIdx.x : warp; sl_i < S::kSlices; sl_i += SPLIT ? S::kSlices : 8) {
+        const int j = sl_i / (HD / 16), i = sl_i % (HD / 16), col = 8 * j + 2 * t4;
+        const bool in = row0 + col < w.rows;
+        // the largest m of each of the lane's two columns
+        float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (in) {
+            for (int n = g; n < parts; n += 8) {
+                const float *p = n == 0 ? first : rest + (int64_t)n * 2 * S::kPart;
+                m[0] = fmaxf(m[0], p[col]);
+                m[1] = fmaxf(m[1], p[col + 1]);
+            }
+        }
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = 0.0f;
-        for (int64_t c = c0 + (SPLIT ? warp : 0); c <= c1; c += SPLIT ? 8 : 1) {
-            const int64_t from = c * all / share, to = (c + 1) * all / share;
-            if (from == to) continue;  // a CTA without work
-            const float *p = a.parts + (c * 2 + (from >= s ? 0 : 1)) * S::kPart;
-            const float pm = p[col], pl = p[kCols + col];
-            float pv[V];
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int i = 0; i < V; ++i) pv[i] = p[2 * kCols + col * HD + i * 32 + lane];
-            const float mn = fmaxf(m, pm), x = ex2(m - mn), y = ex2(pm - mn);
-            m = mn;
-            l = l * x + pl * y;
+            for (int d = 4; d < 32; d <<= 1) m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], d));
+        if (in) {
+            constexpr int U = 4;  // parts in flight
+            for (int n0 = SPLIT ? warp : 0; n0 < parts; n0 += SPLIT ? 8 * U : U) {
+                float4 v[U];
+                float pm[U][2], pl[U][2];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = o[i] * x + pv[i] * y;
+                for (int x = 0; x < U; ++x) {
+                    const int n = n0 + (SPLIT ? 8 * x : x);
+                    const float *p = n == 0 ? first : rest + (int64_t)n * 2 * S::kPart;
+                    pm[x][0] = pm[x][1] = -INFINITY;
+                    if (n < parts) {
+                        v[x] = reinterpret_cast<const float4 *>(p + 2 * kCols)[sl_i * 32 + lane];
+                        pm[x][0] = p[col], pm[x][1] = p[col + 1];
+                        pl[x][0] = p[kCols + col], pl[x][1] = p[kCols + col + 1];
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < U; ++x) {
+                    if (n0 + (SPLIT ? 8 * x : x) < parts) {
+                        const float c = ex2(pm[x][0] - m[0]), d = ex2(pm[x][1] - m[1]);
+                        l[0] = fmaf(c, pl[x][0], l[0]);
+                        l[1] = fmaf(d, pl[x][1], l[1]);
+                        o.x = fmaf(c, v[x].x, o.x), o.z = fmaf(c, v[x].z, o.z);
+                        o.y = fmaf(d, v[x].y, o.y), o.w = fmaf(d, v[x].w, o.w);
+                    }
+                }
+            }
         }
         if (SPLIT) {
-            if (lane == 0) {
-                sm[warp] = m;
-                sl[warp] = l;
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) so[warp][i * 32 + lane] = o[i];
+            so[warp][lane] = o;
+            if (g == 0) sl[warp][col] = l[0], sl[warp][col + 1] = l[1];
             __syncthreads();
             if (warp != 0) return;
             for (int k = 1; k < 8; ++k) {
-                const float mn = fmaxf(m, sm[k]), x = ex2(m - mn), y = ex2(sm[k] - mn);
-                m = mn;
-                l = l * x + sl[k] * y;
-#pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = o[i] * x + so[k][i * 32 + lane] * y;
+                l[0] += sl[k][col], l[1] += sl[k][col + 1];
+                o.x += so[k][lane].x, o.y += so[k][lane].y, o.z += so[k][lane].z, o.w += so[k][lane].w;
             }
         }
-        const int n = row0 + col, tk = n / a.ratio;
-        const int64_t row = (int64_t)(w.first + tk) * a.q_heads + head * a.ratio + (n - tk * a.ratio);
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-        for (int i = 0; i < V; ++i) put(static_cast<T *>(a.out) + row * HD + i * 32 + lane, o[i] * inv);
-        if (lane == 0 && a.log_sum != nullptr)
-            a.log_sum[row] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        write_slice<T, HD>(a, w, head, row0 + col, HD / 8 * g + 2 * i, o.x, o.z, m[0], l[0]);
+        write_slice<T, HD>(a, w, head, row0 + col + 1, HD / 8 * g + 2 * i, o.y, o.w, m[1], l[1]);
     }
 }
 
@@ -615,13 +664,7 @@ template <typename T, int HD, int GS, int NT>
 int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
     const int share = share_of<NT>();
     auto kern = stream_kernel<T, HD, GS, NT>;
-    const size_t red = (size_t)kWarps * Shape<HD, NT>::kPart * 4;
-    const size_t ring = ring_bytes<HD, GS>() > red ? ring_bytes<HD, GS>() : red;
-    // the prefix follows the ring
-    const size_t smem = ring_bytes<HD, GS>() + (batch->sequences + 1) * 8 > ring
-                            ? ring_bytes<HD, GS>() + (batch->sequences + 1) * 8
-                            : ring;
-    static_assert(ring_bytes<HD, GS>() >= (size_t)kWarps * Shape<HD, NT>::kPart * 4, "the join fits the ring");
+    const size_t smem = ring_bytes<HD, GS>() + (batch->sequences + 1) * 8;  // the prefix follows the rings
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void *>(kern), smem)) return rc;
     kern<<<share, kWarps * 32, smem, st>>>(a);
     if (int rc = check_launch("kv4_attention")) return rc;
@@ -629,9 +672,10 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;
     const int64_t blocks = cdiv(most < a.few ? most : a.few, 8 * NT), items = blocks * a.kv_heads;
     OQ_REQUIRE(items <= 65535, "kv4_attention: too many key heads");
-    const bool split = (int64_t)share > 16 * items * batch->sequences;
+    const int warps = share * kWarps;
+    const bool split = warps > 16 * items * batch->sequences;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(split ? 8 * NT : 1, (unsigned)items, batch->sequences);
+    cfg.gridDim = dim3(split ? Shape<HD, NT>::kSlices : 1, (unsigned)items, batch->sequences);
     cfg.blockDim = dim3(256);
     cfg.stream = st;
     cudaLaunchAttribute attr[1];
@@ -639,8 +683,8 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t err = split ? cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, true>, a, share)
-                            : cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, false>, a, share);
+    cudaError_t err = split ? cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, true>, a, warps)
+                            : cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, false>, a, warps);
     if (err != cudaSuccess) {
         set_error("kv4_attention (join): launch failed: %s", cudaGetErrorString(err));
         return OQ_ERR_CUDA;
@@ -680,7 +724,7 @@ extern "C" int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache, c
     if (check_cache(cache) || check_batch(batch, 1) || check_heads(cache, q_heads)) return 0;
     const int nt = columns_of(cache, batch, q_heads);
     const int64_t share = nt == 1 ? share_of<1>() : share_of<2>();
-    return (int64_t)header_bytes(batch) + share * 2 * 8 * nt * (cache->head_dim + 2) * 4;
+    return (int64_t)header_bytes(batch) + share * kWarps * 2 * (16 * nt + nt * cache->head_dim * 8) * 4;
 }
 
 extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *batch, const void *q, int dtype,
