@@ -36,7 +36,7 @@ int check_batch(const oq_kv4_batch *b, int64_t tokens) {
 namespace {
 
 constexpr int kWarps = 4;  // warps per CTA
-constexpr int kRows = 4;   // head rows a lane has in flight
+constexpr int kRows = 4;   // head rows of a lane in one step (and as many in flight)
 
 struct Rotary {
     const float *table;
@@ -51,6 +51,18 @@ struct Rows {  // [tokens][heads][head_dim] with strides in elements
     int64_t ts, hs;
 };
 
+// How a lane finds the partners of its eight elements.
+enum Pairs {
+    kNone,     // no rotation
+    kShuffle,  // half layout, dim / 2 a multiple of 8: eight elements of one other lane
+    kAny,      // interleaved (the lane's own neighbours) or any other half layout (from memory)
+};
+
+int pairs_of(const Rotary &r) {
+    if (r.table == nullptr) return kNone;
+    return !(r.flags & OQ_ROTARY_INTERLEAVED) && r.dim % 16 == 0 ? kShuffle : kAny;
+}
+
 __device__ __forceinline__ int64_t position_at(const Rotary &r, int64_t t) {
     return r.wide ? __ldg(static_cast<const long long *>(r.positions) + t)
                   : (int64_t)__ldg(static_cast<const int *>(r.positions) + t);
@@ -64,21 +76,30 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
     return __float2bfloat16_rn(v);
 }
 
-// Eight consecutive elements as fp32; VEC: 16-byte aligned.  Plain loads (not
-// the read-only path): the output may be the input.
+// Eight consecutive elements as they are in memory.
+template <typename T>
+struct alignas(16) Eight {
+    T e[8];
+};
+
+// VEC: 16-byte aligned.  Plain loads (not the read-only path): the output may
+// be the input.
 template <typename T, bool VEC>
-__device__ __forceinline__ void load_row8(const T *p, float (&v)[8]) {
-    alignas(16) T e[8];
+__device__ __forceinline__ void load_row8(const T *p, Eight<T> &v) {
     if (VEC) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i)
-            reinterpret_cast<uint4 *>(e)[i] = reinterpret_cast<const uint4 *>(p)[i];
+            reinterpret_cast<uint4 *>(v.e)[i] = reinterpret_cast<const uint4 *>(p)[i];
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = p[i];
+        for (int i = 0; i < 8; ++i) v.e[i] = p[i];
     }
+}
+
+template <typename T>
+__device__ __forceinline__ void widen(const Eight<T> &v, float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = Elem<T>::to_f32(e[i]);
+    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f32(v.e[i]);
 }
 
 template <typename T, bool VEC>
@@ -102,15 +123,17 @@ __device__ __forceinline__ void store_row8(T *p, const float (&v)[8]) {
 struct Turn {
     float cs[8], sn[8];
     bool any;  // one of the eight is rotated
+    int src;   // kShuffle: the partners' lane
 };
 
+template <int PAIRS>
 __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, Turn &t) {
-    const int half = r.dim >> 1;
-    const bool inter = r.flags & OQ_ROTARY_INTERLEAVED;
+    const int half = r.dim >> 1, lane = threadIdx.x & 31;
     const float sign = (r.flags & OQ_ROTARY_INVERSE) ? -1.0f : 1.0f;
     const float *row = r.table + pos * r.dim;
     t.any = 8 * c < r.dim;
-    if (!inter && (half & 7) == 0) {
+    if (PAIRS == kShuffle) {
+        t.src = !t.any ? lane : (8 * c < half ? lane + (half >> 3) : lane - (half >> 3));
         if (t.any) {
             const int i0 = 8 * c < half ? 8 * c : 8 * c - half;
             const float s = 8 * c < half ? -sign : sign;
@@ -124,6 +147,7 @@ __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, T
         }
         return;
     }
+    const bool inter = r.flags & OQ_ROTARY_INTERLEAVED;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int i = 8 * c + e;
@@ -145,35 +169,33 @@ __device__ __forceinline__ float turn1(float x, float cs, float partner, float s
 }
 
 // Rotates a lane's eight elements.  All lanes of the warp take part; `row` is
-// the head's first element for partners that no lane's chunk lines up with.
-template <typename T>
-__device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T *row, bool active, int c, float (&x)[8]) {
-    const int half = r.dim >> 1;
-    if (r.flags & OQ_ROTARY_INTERLEAVED) {
-        if (t.any) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float a = x[e], b = x[e + 1];
-                if (8 * c + e < r.dim) {
-                    x[e] = turn1(a, t.cs[e], b, t.sn[e]);
-                    x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
-                }
-            }
-        }
-    } else if ((half & 7) == 0) {
-        const int lane = threadIdx.x & 31, step = half >> 3;
-        const int src = !t.any ? lane : (8 * c < half ? lane + step : lane - step);
+// the head's first element (nullptr: no head).
+template <typename T, int PAIRS>
+__device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T *row, int c, float (&x)[8]) {
+    if (PAIRS == kShuffle) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const float p = __shfl_sync(0xffffffffu, x[e], src);
+            const float p = __shfl_sync(0xffffffffu, x[e], t.src);
             if (t.any) x[e] = turn1(x[e], t.cs[e], p, t.sn[e]);
+        }
+        return;
+    }
+    const int half = r.dim >> 1;
+    if (r.flags & OQ_ROTARY_INTERLEAVED) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const float a = x[e], b = x[e + 1];
+            if (8 * c + e < r.dim) {
+                x[e] = turn1(a, t.cs[e], b, t.sn[e]);
+                x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
+            }
         }
     } else {
         float p[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const int i = 8 * c + e;
-            p[e] = (active && i < r.dim) ? Elem<T>::to_f32(row[i < half ? i + half : i - half]) : 0.0f;
+            p[e] = (row != nullptr && i < r.dim) ? Elem<T>::to_f32(row[i < half ? i + half : i - half]) : 0.0f;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -185,43 +207,52 @@ __device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T 
 //
 // HBM bound: every element is read and written once and needs 3 flops.  A
 // lane owns eight consecutive elements of a head (16 bytes of a 16-bit type),
-// head_dim / 8 lanes a head, and a warp takes kRows rounds of 32 * 8 /
-// head_dim heads of ONE token: its cos and sin are loaded once into registers
-// for all of them, and the partner of an element comes from another lane by
-// shuffle (half layout) or is the lane's own neighbour (interleaved).
-template <typename T, bool VEC>
+// head_dim / 8 lanes a head; a round is the 32 * 8 / head_dim heads that a
+// warp takes at once.  A warp walks rounds of ONE token, kRows at a time with
+// the next kRows in flight: the token's cos and sin are loaded once into
+// registers for all of them, and the partner of an element comes from another
+// lane by shuffle (half layout) or is the lane's own neighbour (interleaved).
+template <typename T, bool VEC, int PAIRS>
 __global__ void __launch_bounds__(kWarps * 32)
 rotary_kernel(Rows x, T *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim, Rotary rot,
-              int parts) {
+              int parts, int rounds) {
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int64_t t = unit / parts;
     if (t >= tokens) return;
     const int lpr = head_dim >> 3, per = 32 / lpr;  // lanes a head, heads a round
     const int sub = lane / lpr, c = lane - sub * lpr;
-    const int h0 = (int)(unit - t * parts) * kRows * per + sub;
+    const int round0 = (int)(unit - t * parts) * rounds;
     const T *xt = static_cast<const T *>(x.p) + t * x.ts;
-    const int64_t pos = position_at(rot, t);
-    float v[kRows][8];
+    const int last = min((round0 + rounds) * per, heads);  // heads [round0 * per, last)
+    auto row_of = [&](int round) {
+        const int h = round * per + sub;
+        return sub < per && h < last ? xt + h * x.hs : nullptr;
+    };
+    Eight<T> next[kRows];
+    auto fetch = [&](int round) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int h = h0 + i * per;
-        if (sub < per && h < heads) load_row8<T, VEC>(xt + h * x.hs + 8 * c, v[i]);
-    }
+        for (int i = 0; i < kRows; ++i)
+            if (const T *p = row_of(round + i)) load_row8<T, VEC>(p + 8 * c, next[i]);
+    };
+    fetch(round0);
+    const int64_t pos = position_at(rot, t);
     const bool ok = pos >= 0 && pos < rot.rows;
     if (!ok && lane == 0) index_error();
     Turn turn;
-    load_turn(rot, ok ? pos : 0, c, turn);
+    load_turn<PAIRS>(rot, ok ? pos : 0, c, turn);
+    for (int round = round0; round * per < last; round += kRows) {
+        float v[kRows][8];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int h = h0 + i * per;
-        rotate8<T>(rot, turn, xt + h * x.hs, sub < per && h < heads, c, v[i]);
-    }
-    __syncwarp();  // y may be x: every lane's loads (partners too) come before any store of the warp
+        for (int i = 0; i < kRows; ++i) widen(next[i], v[i]);
+        if (rounds > kRows) fetch(round + kRows);
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int h = h0 + i * per;
-        if (ok && sub < per && h < heads) store_row8<T, VEC>(y + t * y_ts + h * y_hs + 8 * c, v[i]);
+        for (int i = 0; i < kRows; ++i) rotate8<T, PAIRS>(rot, turn, row_of(round + i), c, v[i]);
+        __syncwarp();  // y may be x: partners are read before any store of the warp
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (ok && row_of(round + i))
+                store_row8<T, VEC>(y + t * y_ts + ((round + i) * per + sub) * y_hs + 8 * c, v[i]);
     }
 }
 
@@ -233,22 +264,51 @@ __device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, in
     int first, count;
     tokens_of(bt, seq, tokens, first, count);
     if (t < first || t >= first + count) return false;
-    pos = (int64_t)length_of(bt, seq, page_size) - count + (t - first);
-    if (pos >= 0) {
-        const int page = __ldg(bt.table + (int64_t)seq * bt.max_pages + pos / page_size);
-        if (page >= 0 && page < pages) at = ((int64_t)page * kv_heads) * page_size + pos % page_size;
+    const int p = length_of(bt, seq, page_size) - count + (int)(t - first);
+    pos = p;
+    if (p >= 0) {
+        const int slot = p / page_size, page = __ldg(bt.table + (int64_t)seq * bt.max_pages + slot);
+        if (page >= 0 && page < pages) at = ((int64_t)page * kv_heads) * page_size + (p - slot * page_size);
     }
     if (at < 0 && (threadIdx.x & 31) == 0) index_error();
     return true;
 }
 
+// The codes of eight elements as a word: clip(rint(fl(x / s)), -7, 7) with
+// fl() the IEEE quotient.  r = x * (1 / s) is within 2e-6 of it where the
+// clipped range is not left, so both round to the same integer unless r is
+// that near to a half; then (1 in 10^5) and beyond the range every element
+// takes the division.  Adding 1.5 * 2^23 + 8 leaves u = code + 8 in the low
+// bits of 0x4B400000 + u; the eight sums shifted by 4 e add up, and the
+// constants' own sum is 0x3F400000 (mod 2^32).
+__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float s) {
+    constexpr float kMagic = kRoundMagic + 8.0f;
+    const float inv = __fdiv_rn(1.0f, s);
+    uint32_t acc = 0;
+    bool slow = false;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+        const float r = __fmul_rn(x[e], inv), t = __fadd_rn(r, kMagic), n = __fsub_rn(t, kMagic);
+        slow |= !(fabsf(__fsub_rn(r, n)) < 0.49999f && fabsf(n) <= 7.0f);
+        acc = acc * 16 + __float_as_uint(t);
+    }
+    if (slow) {
+        acc = 0;
+#pragma unroll
+        for (int e = 7; e >= 0; --e)
+            acc = acc * 16 +
+                  __float_as_uint(__fadd_rn(fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -7.0f), 7.0f), kMagic));
+    }
+    return (acc - 0x3F400000u) ^ 0x88888888u;
+}
+
 // ------------------------------------------------------------- append ----
 //
-// HBM bound at many tokens, latency bound at a few.  The same lane layout as
-// the rotary kernel, over the token's query heads and then its key and value
-// heads in pairs (k0 v0 k1 v1 ...), so that a key and the value that goes
-// with it sit in neighbouring lane groups of one round.  A group's maximum
-// is a shuffle over group / 8 lanes; a lane's eight codes are one word.
+// HBM bound at many tokens, latency bound at a few.  The same lane layout and
+// walk as the rotary kernel, over the token's query heads and then its key
+// and value heads in pairs (k0 v0 k1 v1 ...), so that a key and the value that
+// goes with it sit in neighbouring lane groups of one round.  A group's
+// maximum is a shuffle over group / 8 lanes; a lane's eight codes are one word.
 struct AppendArgs {
     Rows q, k, v;
     void *q_out;
@@ -257,109 +317,116 @@ struct AppendArgs {
     uint32_t *k_codes, *v_codes;
     __half *k_scales, *v_scales;
     int64_t pages, tokens;
-    int parts, q_rounds;
-    Rotary rot;  // table nullptr: no rotation
+    int parts, rounds, q_rounds, all_rounds;  // rounds a warp; of the queries; of a token
+    Rotary rot;                               // table nullptr: no rotation
     Batch batch;
 };
 
-template <typename T, int D, bool VEC>
-__global__ void __launch_bounds__(kWarps * 32) append_kernel(AppendArgs a) {
+template <typename T, int D, bool VEC, int PAIRS>
+__global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int LPR = D / 8, PER = 32 / LPR;
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
     const int64_t t = unit / a.parts;
     if (t >= a.tokens) return;
     const int sub = lane / LPR, c = lane % LPR;
-    const int round0 = (int)(unit - t * a.parts) * kRows;
+    const int round0 = (int)(unit - t * a.parts) * a.rounds, round1 = min(round0 + a.rounds, a.all_rounds);
     const int kv_rows = 2 * a.kv_heads;
 
-    // row of round i: [0, q_heads) a query head; a key or value head after
-    // the rounds of the queries
-    float x[kRows][8];
-    const T *src[kRows];
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int round = round0 + i;
-        src[i] = nullptr;
+    // This lane's head row of a round (nullptr: none): a query head, and after
+    // the rounds of the queries a key or value head.
+    auto row_of = [&](int round) -> const T * {
+        if (round >= round1) return nullptr;
         if (round < a.q_rounds) {
             const int h = round * PER + sub;
-            if (h < a.q_heads) src[i] = static_cast<const T *>(a.q.p) + t * a.q.ts + h * a.q.hs;
-        } else {
-            const int row = (round - a.q_rounds) * PER + sub;
-            if (row < kv_rows) {
-                const Rows &m = (row & 1) ? a.v : a.k;
-                src[i] = static_cast<const T *>(m.p) + t * m.ts + (row >> 1) * m.hs;
-            }
+            return h < a.q_heads ? static_cast<const T *>(a.q.p) + t * a.q.ts + h * a.q.hs : nullptr;
         }
+        const int row = (round - a.q_rounds) * PER + sub;
+        if (row >= kv_rows) return nullptr;
+        const Rows &m = (row & 1) ? a.v : a.k;
+        return static_cast<const T *>(m.p) + t * m.ts + (row >> 1) * m.hs;
+    };
+    Eight<T> next[kRows];
+    auto fetch = [&](int round) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-        if (src[i] != nullptr) load_row8<T, VEC>(src[i] + 8 * c, x[i]);
-    }
+        for (int i = 0; i < kRows; ++i)
+            if (const T *p = row_of(round + i)) load_row8<T, VEC>(p + 8 * c, next[i]);
+    };
+    fetch(round0);
 
     const int seq = sequence_of(a.batch, (int)t);
     int64_t pos = 0, at = -1;  // place in the sequence; row of head 0 in the cache
     const bool real = find_row(a.batch, seq, t, a.tokens, a.pages, a.page_size, a.kv_heads, pos, at);
-    int64_t angle = a.rot.positions != nullptr ? position_at(a.rot, t) : pos;
-    const bool turned = a.rot.table != nullptr;
-    const bool ok = !turned || (angle >= 0 && angle < a.rot.rows);
+    const int64_t angle = PAIRS != kNone && a.rot.positions != nullptr ? position_at(a.rot, t) : pos;
+    const bool ok = PAIRS == kNone || (angle >= 0 && angle < a.rot.rows);
     if (!ok && real && lane == 0) index_error();
     Turn turn;
-    if (turned) load_turn(a.rot, ok ? angle : 0, c, turn);
+    if (PAIRS != kNone) load_turn<PAIRS>(a.rot, ok ? angle : 0, c, turn);
 
+    for (int round = round0; round < round1; round += kRows) {
+        float x[kRows][8];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int round = round0 + i;
-        if (round < a.q_rounds) {  // warp-uniform
-            if (turned) rotate8<T>(a.rot, turn, src[i], src[i] != nullptr, c, x[i]);
-            __syncwarp();  // q_out may be q
-            if (src[i] != nullptr && ok)
-                store_row8<T, VEC>(static_cast<T *>(a.q_out) + t * a.qo_ts + (round * PER + sub) * a.qo_hs + 8 * c,
-                                   x[i]);
-            continue;
-        }
-        const int row = (round - a.q_rounds) * PER + sub;
-        const bool is_v = row & 1;
-        if (turned) {
-            float y[8];
+        for (int i = 0; i < kRows; ++i) widen(next[i], x[i]);
+        if (a.rounds > kRows) fetch(round + kRows);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[i][e];
-            rotate8<T>(a.rot, turn, src[i], src[i] != nullptr, c, y);
+        for (int i = 0; i < kRows; ++i) {
+            const int rd = round + i;
+            const T *src = row_of(rd);
+            if (rd < a.q_rounds) {  // warp-uniform
+                if (PAIRS != kNone) rotate8<T, PAIRS>(a.rot, turn, src, c, x[i]);
+                __syncwarp();  // q_out may be q
+                if (src != nullptr && ok)
+                    store_row8<T, VEC>(static_cast<T *>(a.q_out) + t * a.qo_ts + (rd * PER + sub) * a.qo_hs + 8 * c,
+                                       x[i]);
+                continue;
+            }
+            if (rd >= round1) continue;
+            const int row = (rd - a.q_rounds) * PER + sub;
+            const bool is_v = row & 1;
+            if (src == nullptr) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[i][e] = is_v ? x[i][e] : y[e];
-        }
-        float mx = 0.0f;
+                for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
+            }
+            if (PAIRS != kNone) {
+                float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx = nan_max(mx, fabsf(x[i][e]));
-        // Not finite anywhere in the token's key or value of this head: the
-        // lanes of both (2 * LPR of them) agree on it.
-        const unsigned bad_lanes = __ballot_sync(0xffffffffu, !(mx <= 3.402823466e38f));
-        const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
-        const bool bad = (bad_lanes & pair) != 0;
-        for (int o = 0; o < a.group_log; ++o) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
-        __half s16 = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(mx, 7.0f))));
-        float s = fminf(__half2float(s16), kMaxScale);
-        if (s == 0.0f || bad) s = 1.0f;
-        const float inv = __fdiv_rn(1.0f, s);
-        uint32_t word = 0;
+                for (int e = 0; e < 8; ++e) y[e] = x[i][e];
+                rotate8<T, PAIRS>(a.rot, turn, src, c, y);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) word |= (quant_bits(x[i][e], s, inv, 7.0f) & 15u) << (4 * e);
-        if (bad) word = 0;
-        if (row < kv_rows && at >= 0 && ok) {
-            const int64_t r = at + (int64_t)(row >> 1) * a.page_size;
-            (is_v ? a.v_codes : a.k_codes)[r * (D / 8) + c] = word;
-            if ((c & ((1 << a.group_log) - 1)) == 0)
-                (is_v ? a.v_scales : a.k_scales)[r * (LPR >> a.group_log) + (c >> a.group_log)] =
-                    bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
+                for (int e = 0; e < 8; ++e) x[i][e] = is_v ? x[i][e] : y[e];
+            }
+            float mx = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) mx = nan_max(mx, fabsf(x[i][e]));
+            // Not finite anywhere in the token's key or value of this head: the
+            // lanes of both (2 * LPR of them) agree on it.
+            const unsigned bad_lanes = __ballot_sync(0xffffffffu, !(mx <= 3.402823466e38f));
+            const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
+            const bool bad = (bad_lanes & pair) != 0;
+            for (int o = 0; o < a.group_log; ++o) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
+            const __half s16 = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(mx, 7.0f))));
+            float s = fminf(__half2float(s16), kMaxScale);
+            if (s == 0.0f || bad) s = 1.0f;
+            const uint32_t word = bad ? 0u : pack8(x[i], s);
+            if (row < kv_rows && at >= 0 && ok) {
+                const int64_t r = at + (int64_t)(row >> 1) * a.page_size;
+                (is_v ? a.v_codes : a.k_codes)[r * (D / 8) + c] = word;
+                if ((c & ((1 << a.group_log) - 1)) == 0)
+                    (is_v ? a.v_scales : a.k_scales)[r * (LPR >> a.group_log) + (c >> a.group_log)] =
+                        bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
+            }
         }
     }
 }
 
 // --------------------------------------------------------------- read ----
-
+//
+// HBM bound; the walk of the append kernel over the key and value heads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32)
 read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_codes, const __half *v_scales, T *k,
-            T *v, Batch batch, int64_t pages, int page_size, int kv_heads, int group_log, int64_t tokens, int parts) {
+            T *v, Batch batch, int64_t pages, int page_size, int kv_heads, int group_log, int64_t tokens, int parts,
+            int rounds) {
     constexpr int LPR = D / 8, PER = 32 / LPR;
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -369,30 +436,54 @@ read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_c
     const int seq = sequence_of(batch, (int)t);
     int64_t pos = 0, at = -1;
     find_row(batch, seq, t, tokens, pages, page_size, kv_heads, pos, at);
-    const int row0 = (int)(unit - t * parts) * kRows * PER + sub;
-    uint32_t word[kRows];
-    __half sc[kRows];
+    const int row0 = (int)(unit - t * parts) * rounds * PER + sub;
+    const int row1 = min(row0 + rounds * PER, 2 * kv_heads);
+    uint32_t next[kRows];
+    __half scale[kRows];
+    auto fetch = [&](int row_) {
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int row = row0 + i * PER;
-        word[i] = 0;
-        sc[i] = __ushort_as_half(0);
-        if (at >= 0 && row < 2 * kv_heads) {
-            const int64_t r = at + (int64_t)(row >> 1) * page_size;
-            word[i] = ((row & 1) ? v_codes : k_codes)[r * (D / 8) + c];
-            sc[i] = ((row & 1) ? v_scales : k_scales)[r * (LPR >> group_log) + (c >> group_log)];
+        for (int i = 0; i < kRows; ++i) {
+            const int row = row_ + i * PER;
+            next[i] = 0;
+            scale[i] = __ushort_as_half(0);
+            if (at >= 0 && row < row1) {
+                const int64_t r = at + (int64_t)(row >> 1) * page_size;
+                next[i] = ((row & 1) ? v_codes : k_codes)[r * (D / 8) + c];
+                scale[i] = ((row & 1) ? v_scales : k_scales)[r * (LPR >> group_log) + (c >> group_log)];
+            }
+        }
+    };
+    fetch(row0);
+    for (int row_ = row0; row_ < row1; row_ += kRows * PER) {
+        uint32_t word[kRows];
+        float s[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            word[i] = next[i];
+            s[i] = __half2float(scale[i]);
+        }
+        if (rounds > kRows) fetch(row_ + kRows * PER);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int row = row_ + i * PER;
+            if (row >= row1) continue;
+            float o[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = (float)nibble_value(word[i] >> (8 * (e >> 1)), e & 1) * s[i];
+            store_row8<T, true>(((row & 1) ? v : k) + ((int64_t)t * kv_heads + (row >> 1)) * D + 8 * c, o);
         }
     }
-#pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int row = row0 + i * PER;
-        if (row >= 2 * kv_heads) continue;
-        const float s = __half2float(sc[i]);
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = (float)nibble_value(word[i] >> (8 * (e >> 1)), e & 1) * s;
-        store_row8<T, true>(((row & 1) ? v : k) + ((int64_t)t * kv_heads + (row >> 1)) * D + 8 * c, o);
-    }
+}
+
+// Rounds a warp takes of a token that has `all`: as many as leave the GPU
+// kFill warps a SM, in steps of kRows.  (Few: a warp's lookups are paid for
+// more often; many: too few warps at small sizes.)
+constexpr int kFill = 32;
+
+int rounds_of(int64_t tokens, int64_t all) {
+    const int64_t want = tokens * all / ((int64_t)sm_count() * kFill);
+    const int64_t r = want / kRows * kRows;
+    return (int)(r < kRows ? kRows : (r > all ? cdiv(all, kRows) * kRows : r));
 }
 
 int check_rotary(const oq_rotary_spec *r, int head_dim) {
@@ -410,41 +501,51 @@ int grid_of(int64_t units, int64_t *blocks) {
     return OQ_OK;
 }
 
+template <typename T, bool VEC>
+void rotary_start(const Rows &x, void *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim,
+                  const Rotary &rot, int parts, int rounds, unsigned blocks, cudaStream_t st) {
+    auto kern = pairs_of(rot) == kShuffle ? rotary_kernel<T, VEC, kShuffle> : rotary_kernel<T, VEC, kAny>;
+    kern<<<blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens, heads, head_dim, rot, parts,
+                                         rounds);
+}
+
 template <typename T>
 int rotary_launch(const Rows &x, void *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim,
                   const Rotary &rot, cudaStream_t st) {
-    const int per = 32 / (head_dim / 8);
-    const int parts = (int)cdiv(heads, kRows * per);
+    const int64_t all = cdiv(heads, 32 / (head_dim / 8));
+    const int rounds = rounds_of(tokens, all), parts = (int)cdiv(all, rounds);
     int64_t blocks;
     if (int rc = grid_of(tokens * parts, &blocks)) return rc;
     const int64_t n = 16 / sizeof(T);
     const bool vec = aligned(x.p, 16) && aligned(y, 16) && x.ts % n == 0 && x.hs % n == 0 && y_ts % n == 0 &&
                      y_hs % n == 0;
-    if (vec)
-        rotary_kernel<T, true><<<(unsigned)blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens,
-                                                                         heads, head_dim, rot, parts);
-    else
-        rotary_kernel<T, false><<<(unsigned)blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens,
-                                                                          heads, head_dim, rot, parts);
+    (vec ? rotary_start<T, true> : rotary_start<T, false>)(x, y, y_ts, y_hs, tokens, heads, head_dim, rot, parts,
+                                                           rounds, (unsigned)blocks, st);
     return check_launch("rotary");
+}
+
+template <typename T, int D, bool VEC>
+void append_start(const AppendArgs &a, unsigned blocks, cudaStream_t st) {
+    const int pairs = pairs_of(a.rot);
+    auto kern = pairs == kNone      ? append_kernel<T, D, VEC, kNone>
+                : pairs == kShuffle ? append_kernel<T, D, VEC, kShuffle>
+                                    : append_kernel<T, D, VEC, kAny>;
+    kern<<<blocks, kWarps * 32, 0, st>>>(a);
 }
 
 template <typename T, int D>
 int append_launch(const AppendArgs &a, bool vec, int64_t blocks, cudaStream_t st) {
-    if (vec)
-        append_kernel<T, D, true><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a);
-    else
-        append_kernel<T, D, false><<<(unsigned)blocks, kWarps * 32, 0, st>>>(a);
+    (vec ? append_start<T, D, true> : append_start<T, D, false>)(a, (unsigned)blocks, st);
     return check_launch("kv4_append");
 }
 
 template <typename T, int D>
 int read_launch(const oq_kv4_cache *c, const Batch &b, void *k, void *v, int group_log, int64_t tokens, int parts,
-                int64_t blocks, cudaStream_t st) {
+                int rounds, int64_t blocks, cudaStream_t st) {
     read_kernel<T, D><<<(unsigned)blocks, kWarps * 32, 0, st>>>(
         reinterpret_cast<const uint32_t *>(c->k_codes), static_cast<const __half *>(c->k_scales),
         reinterpret_cast<const uint32_t *>(c->v_codes), static_cast<const __half *>(c->v_scales), static_cast<T *>(k),
-        static_cast<T *>(v), b, c->pages, c->page_size, c->kv_heads, group_log, tokens, parts);
+        static_cast<T *>(v), b, c->pages, c->page_size, c->kv_heads, group_log, tokens, parts, rounds);
     return check_launch("kv4_read");
 }
 
@@ -510,7 +611,9 @@ extern "C" int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batc
     a.tokens = tokens;
     const int per = 32 / (cache->head_dim / 8);
     a.q_rounds = (int)cdiv(a.q_heads, per);
-    a.parts = (int)cdiv(a.q_rounds + cdiv(2 * a.kv_heads, per), kRows);
+    a.all_rounds = a.q_rounds + (int)cdiv(2 * a.kv_heads, per);
+    a.rounds = rounds_of(tokens, a.all_rounds);
+    a.parts = (int)cdiv(a.all_rounds, a.rounds);
     if (rotary != nullptr)
         a.rot = Rotary{rotary->table, rotary->rows, rotary->dim, rotary->flags, positions, positions_64};
     a.batch = device_batch(batch);
@@ -537,7 +640,8 @@ extern "C" int oq_kv4_read(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
     OQ_REQUIRE(k && v, "null pointer argument");
     OQ_REQUIRE(aligned(k, 16) && aligned(v, 16), "kv4_read: k and v must be 16-byte aligned");
     const int per = 32 / (cache->head_dim / 8);
-    const int parts = (int)cdiv(2 * cache->kv_heads, kRows * per);
+    const int64_t all = cdiv(2 * cache->kv_heads, per);
+    const int rounds = rounds_of(tokens, all), parts = (int)cdiv(all, rounds);
     int64_t blocks;
     if (int rc = grid_of(tokens * parts, &blocks)) return rc;
     const int gl = group_log_of(cache->group_size);
@@ -545,11 +649,11 @@ extern "C" int oq_kv4_read(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool d64 = cache->head_dim == 64;
     if (dtype == OQ_F32)
-        return d64 ? read_launch<float, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
-                   : read_launch<float, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
+        return d64 ? read_launch<float, 64>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st)
+                   : read_launch<float, 128>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st);
     if (dtype == OQ_F16)
-        return d64 ? read_launch<__half, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
-                   : read_launch<__half, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
-    return d64 ? read_launch<__nv_bfloat16, 64>(cache, b, k, v, gl, tokens, parts, blocks, st)
-               : read_launch<__nv_bfloat16, 128>(cache, b, k, v, gl, tokens, parts, blocks, st);
+        return d64 ? read_launch<__half, 64>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st)
+                   : read_launch<__half, 128>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st);
+    return d64 ? read_launch<__nv_bfloat16, 64>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st)
+               : read_launch<__nv_bfloat16, 128>(cache, b, k, v, gl, tokens, parts, rounds, blocks, st);
 }
