@@ -486,8 +486,8 @@ OQ_API int oq_rotary(const void *x, void *y, int dtype, int64_t tokens,
 
 /* Writes a step's keys and values into the cache, in one kernel: k is rotated
  * (rotary NULL: taken as it is) in fp32 and quantized without another
- * rounding, v is quantized, and q, when not NULL, is rotated into q_out
- * (which may be q).  k, v [tokens][kv_heads][head_dim] and q
+ * rounding, v is quantized, and q, when not NULL (which needs rotary), is
+ * rotated into q_out (which may be q).  k, v [tokens][kv_heads][head_dim] and q
  * [tokens][q_heads][head_dim] are fp16 or bf16, strides in elements, a head
  * contiguous.  positions (int32 / int64 [tokens]) replaces the tokens' places
  * in their sequences for the rotation only; NULL: those places. */

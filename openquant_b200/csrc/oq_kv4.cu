@@ -55,12 +55,14 @@ struct Rows {  // [tokens][heads][head_dim] with strides in elements
 enum Pairs {
     kNone,     // no rotation
     kShuffle,  // half layout, dim / 2 a multiple of 8: eight elements of one other lane
-    kAny,      // interleaved (the lane's own neighbours) or any other half layout (from memory)
+    kNext,     // interleaved, dim a multiple of 8: the lane's own neighbours
+    kAny,      // any other dim: half-layout partners from memory
 };
 
 int pairs_of(const Rotary &r) {
     if (r.table == nullptr) return kNone;
-    return !(r.flags & OQ_ROTARY_INTERLEAVED) && r.dim % 16 == 0 ? kShuffle : kAny;
+    if (r.flags & OQ_ROTARY_INTERLEAVED) return r.dim % 8 == 0 ? kNext : kAny;
+    return r.dim % 16 == 0 ? kShuffle : kAny;
 }
 
 __device__ __forceinline__ int64_t position_at(const Rotary &r, int64_t t) {
@@ -147,6 +149,19 @@ __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, T
         }
         return;
     }
+    if (PAIRS == kNext) {
+        if (t.any) {
+            const float4 a = __ldg(reinterpret_cast<const float4 *>(row + 4 * c));
+            const float4 b = __ldg(reinterpret_cast<const float4 *>(row + half + 4 * c));
+            const float cs[4] = {a.x, a.y, a.z, a.w}, sn[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                t.cs[e] = cs[e >> 1];
+                t.sn[e] = ((e & 1) ? sign : -sign) * sn[e >> 1];
+            }
+        }
+        return;
+    }
     const bool inter = r.flags & OQ_ROTARY_INTERLEAVED;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -180,6 +195,18 @@ __device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T 
         }
         return;
     }
+    if (PAIRS == kNext) {
+        if (t.any) {
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+                const float a = x[e], b = x[e + 1];
+                x[e] = turn1(a, t.cs[e], b, t.sn[e]);
+                x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
+            }
+        }
+        return;
+    }
+    if (!t.any) return;
     const int half = r.dim >> 1;
     if (r.flags & OQ_ROTARY_INTERLEAVED) {
 #pragma unroll
@@ -275,31 +302,47 @@ __device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, in
 }
 
 // The codes of eight elements as a word: clip(rint(fl(x / s)), -7, 7) with
-// fl() the IEEE quotient.  r = x * (1 / s) is within 2e-6 of it where the
+// fl() the IEEE quotient.  r = x * rcp(s) is within 2e-6 of it where the
 // clipped range is not left, so both round to the same integer unless r is
-// that near to a half; then (1 in 10^5) and beyond the range every element
-// takes the division.  Adding 1.5 * 2^23 + 8 leaves u = code + 8 in the low
+// within 1e-5 of a half; then (2 in 10^5), and beyond the range, the word
+// takes the divisions.  Adding 1.5 * 2^23 + 8 leaves u = code + 8 in the low
 // bits of 0x4B400000 + u; the eight sums shifted by 4 e add up, and the
 // constants' own sum is 0x3F400000 (mod 2^32).
-__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float s) {
-    constexpr float kMagic = kRoundMagic + 8.0f;
-    const float inv = __fdiv_rn(1.0f, s);
+constexpr float kMagic = kRoundMagic + 8.0f;
+
+__device__ __noinline__ uint32_t divide8(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
+                                         float s) {
+    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
     uint32_t acc = 0;
-    bool slow = false;
+#pragma unroll
+    for (int e = 7; e >= 0; --e)
+        acc = acc * 16 + __float_as_uint(__fadd_rn(fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -7.0f), 7.0f), kMagic));
+    return acc;
+}
+
+__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float s) {
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    uint32_t acc = 0;
+    float off = 0.0f, big = 0.0f;  // the largest distance from an integer, and the largest integer
 #pragma unroll
     for (int e = 7; e >= 0; --e) {
         const float r = __fmul_rn(x[e], inv), t = __fadd_rn(r, kMagic), n = __fsub_rn(t, kMagic);
-        slow |= !(fabsf(__fsub_rn(r, n)) < 0.49999f && fabsf(n) <= 7.0f);
+        off = fmaxf(off, fabsf(__fsub_rn(r, n)));
+        big = fmaxf(big, fabsf(n));
         acc = acc * 16 + __float_as_uint(t);
     }
-    if (slow) {
-        acc = 0;
-#pragma unroll
-        for (int e = 7; e >= 0; --e)
-            acc = acc * 16 +
-                  __float_as_uint(__fadd_rn(fminf(fmaxf(rintf(__fdiv_rn(x[e], s)), -7.0f), 7.0f), kMagic));
-    }
+    if (off > 0.49999f || big > 7.0f) acc = divide8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s);
     return (acc - 0x3F400000u) ^ 0x88888888u;
+}
+
+// A group's scale: fl(mx / 7) (Markstein's correction of the product with
+// RN(1 / 7), the IEEE quotient of every positive finite mx), 8 bits, fp16.
+__device__ __forceinline__ float scale_of(float mx) {
+    const float y = 0.14285714924335479736f, q = __fmul_rn(mx, y);
+    const float s = fmaf(fmaf(-q, 7.0f, mx), y, q);
+    const float s16 = fminf(__half2float(__float2half_rn(__bfloat162float(__float2bfloat16_rn(s)))), kMaxScale);
+    return s16 == 0.0f ? 1.0f : s16;
 }
 
 // ------------------------------------------------------------- append ----
@@ -331,28 +374,33 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
     if (t >= a.tokens) return;
     const int sub = lane / LPR, c = lane % LPR;
     const int round0 = (int)(unit - t * a.parts) * a.rounds, round1 = min(round0 + a.rounds, a.all_rounds);
-    const int kv_rows = 2 * a.kv_heads;
 
-    // This lane's head row of a round (nullptr: none): a query head, and after
-    // the rounds of the queries a key or value head.
-    auto row_of = [&](int round) -> const T * {
-        if (round >= round1) return nullptr;
-        if (round < a.q_rounds) {
-            const int h = round * PER + sub;
-            return h < a.q_heads ? static_cast<const T *>(a.q.p) + t * a.q.ts + h * a.q.hs : nullptr;
-        }
-        const int row = (round - a.q_rounds) * PER + sub;
-        if (row >= kv_rows) return nullptr;
-        const Rows &m = (row & 1) ? a.v : a.k;
-        return static_cast<const T *>(m.p) + t * m.ts + (row >> 1) * m.hs;
-    };
+    // Rounds [round0, q1) are the queries': the lane's head is round * PER +
+    // sub.  Rounds [kv0, kv1) (counted from the first one after the queries)
+    // are the keys' and values': a lane group has keys only or values only.
+    const int q1 = min(round1, a.q_rounds);
+    const int kv0 = max(round0 - a.q_rounds, 0), kv1 = round1 - a.q_rounds;
+    const bool is_v = sub & 1;
+    const Rows &kv = is_v ? a.v : a.k;
+    const T *q_src = static_cast<const T *>(a.q.p) + t * a.q.ts + sub * a.q.hs + 8 * c;
+    const T *kv_src = static_cast<const T *>(kv.p) + t * kv.ts + (sub >> 1) * kv.hs + 8 * c;
     Eight<T> next[kRows];
-    auto fetch = [&](int round) {
+    auto fetch_q = [&](int round) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-            if (const T *p = row_of(round + i)) load_row8<T, VEC>(p + 8 * c, next[i]);
+            if (round + i < q1 && (round + i) * PER + sub < a.q_heads)
+                load_row8<T, VEC>(q_src + (int64_t)((round + i) * PER) * a.q.hs, next[i]);
     };
-    fetch(round0);
+    auto fetch_kv = [&](int round) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (round + i < kv1 && (round + i) * (PER / 2) + (sub >> 1) < a.kv_heads)
+                load_row8<T, VEC>(kv_src + (int64_t)((round + i) * (PER / 2)) * kv.hs, next[i]);
+    };
+    if (round0 < q1)
+        fetch_q(round0);
+    else
+        fetch_kv(kv0);
 
     const int seq = sequence_of(a.batch, (int)t);
     int64_t pos = 0, at = -1;  // place in the sequence; row of head 0 in the cache
@@ -363,57 +411,66 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
     Turn turn;
     if (PAIRS != kNone) load_turn<PAIRS>(a.rot, ok ? angle : 0, c, turn);
 
-    for (int round = round0; round < round1; round += kRows) {
+    // ---- queries (only with a rotation)
+    if (PAIRS != kNone) {
+        T *dst = static_cast<T *>(a.q_out) + t * a.qo_ts + sub * a.qo_hs + 8 * c;
+        for (int round = round0; round < q1; round += kRows) {
+            float x[kRows][8];
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) widen(next[i], x[i]);
+            if (round + kRows < q1)
+                fetch_q(round + kRows);
+            else
+                fetch_kv(kv0);
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+                const bool in = round + i < q1 && (round + i) * PER + sub < a.q_heads;
+                rotate8<T, PAIRS>(a.rot, turn, in ? q_src + (int64_t)((round + i) * PER) * a.q.hs - 8 * c : nullptr, c,
+                                  x[i]);
+            }
+            __syncwarp();  // q_out may be q: partners are read before any store of the warp
+#pragma unroll
+            for (int i = 0; i < kRows; ++i)
+                if (ok && round + i < q1 && (round + i) * PER + sub < a.q_heads)
+                    store_row8<T, VEC>(dst + (int64_t)((round + i) * PER) * a.qo_hs, x[i]);
+        }
+    }
+
+    // ---- keys and values
+    if (PAIRS != kNone) turn.any = turn.any && !is_v;
+    const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
+    const int lanes = 1 << a.group_log, groups = LPR >> a.group_log;
+    const bool first = (c & (lanes - 1)) == 0;
+    uint32_t *codes = (is_v ? a.v_codes : a.k_codes) + (at + (int64_t)(sub >> 1) * a.page_size) * (D / 8) + c;
+    __half *scales = (is_v ? a.v_scales : a.k_scales) + (at + (int64_t)(sub >> 1) * a.page_size) * groups +
+                     (c >> a.group_log);
+    for (int round = kv0; round < kv1; round += kRows) {
         float x[kRows][8];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) widen(next[i], x[i]);
-        if (a.rounds > kRows) fetch(round + kRows);
+        fetch_kv(round + kRows);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int rd = round + i;
-            const T *src = row_of(rd);
-            if (rd < a.q_rounds) {  // warp-uniform
-                if (PAIRS != kNone) rotate8<T, PAIRS>(a.rot, turn, src, c, x[i]);
-                __syncwarp();  // q_out may be q
-                if (src != nullptr && ok)
-                    store_row8<T, VEC>(static_cast<T *>(a.q_out) + t * a.qo_ts + (rd * PER + sub) * a.qo_hs + 8 * c,
-                                       x[i]);
-                continue;
-            }
-            if (rd >= round1) continue;
-            const int row = (rd - a.q_rounds) * PER + sub;
-            const bool is_v = row & 1;
-            if (src == nullptr) {
+            if (round + i >= kv1) break;  // warp-uniform
+            const int head = (round + i) * (PER / 2) + (sub >> 1);
+            const bool in = head < a.kv_heads;
+            if (PAIRS != kNone)
+                rotate8<T, PAIRS>(a.rot, turn,
+                                  in ? kv_src + (int64_t)((round + i) * (PER / 2)) * kv.hs - 8 * c : nullptr, c, x[i]);
+            // the largest magnitude as its bits: an infinity or a NaN is at least 0x7F800000
+            uint32_t mx = 0;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = 0.0f;
-            }
-            if (PAIRS != kNone) {
-                float y[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = x[i][e];
-                rotate8<T, PAIRS>(a.rot, turn, src, c, y);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) x[i][e] = is_v ? x[i][e] : y[e];
-            }
-            float mx = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) mx = nan_max(mx, fabsf(x[i][e]));
+            for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
             // Not finite anywhere in the token's key or value of this head: the
             // lanes of both (2 * LPR of them) agree on it.
-            const unsigned bad_lanes = __ballot_sync(0xffffffffu, !(mx <= 3.402823466e38f));
-            const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
-            const bool bad = (bad_lanes & pair) != 0;
-            for (int o = 0; o < a.group_log; ++o) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
-            const __half s16 = __float2half_rn(__bfloat162float(__float2bfloat16_rn(__fdiv_rn(mx, 7.0f))));
-            float s = fminf(__half2float(s16), kMaxScale);
-            if (s == 0.0f || bad) s = 1.0f;
+            const bool bad = (__ballot_sync(0xffffffffu, in && mx >= 0x7F800000u) & pair) != 0;
+            for (int o = 0; o < a.group_log; ++o) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
+            const float s = bad ? 1.0f : scale_of(__uint_as_float(mx));
             const uint32_t word = bad ? 0u : pack8(x[i], s);
-            if (row < kv_rows && at >= 0 && ok) {
-                const int64_t r = at + (int64_t)(row >> 1) * a.page_size;
-                (is_v ? a.v_codes : a.k_codes)[r * (D / 8) + c] = word;
-                if ((c & ((1 << a.group_log) - 1)) == 0)
-                    (is_v ? a.v_scales : a.k_scales)[r * (LPR >> a.group_log) + (c >> a.group_log)] =
-                        bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
+            if (in && at >= 0 && ok) {
+                const int64_t row = (int64_t)((round + i) * (PER / 2)) * a.page_size;
+                codes[row * (D / 8)] = word;
+                if (first) scales[row * groups] = bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
             }
         }
     }
@@ -422,6 +479,24 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
 // --------------------------------------------------------------- read ----
 //
 // HBM bound; the walk of the append kernel over the key and value heads.
+template <typename T>
+__device__ __forceinline__ void values8(uint32_t word, __half scale, T (&o)[8]) {
+    __half2 v[4];
+    unpack_int(word, v);  // pairs (i, i + 4)
+    const __half2 s = __half2half2(scale);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[i] = __hmul2(v[i], s);  // exact
+        if constexpr (std::is_same<T, __half>::value) {
+            o[i] = __low2half(v[i]);
+            o[i + 4] = __high2half(v[i]);
+        } else {
+            o[i] = from_f32<T>(__low2float(v[i]));
+            o[i + 4] = from_f32<T>(__high2float(v[i]));
+        }
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32)
 read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_codes, const __half *v_scales, T *k,
@@ -433,44 +508,50 @@ read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_c
     const int64_t t = unit / parts;
     if (t >= tokens) return;
     const int sub = lane / LPR, c = lane % LPR;
+    const bool is_v = sub & 1;  // a lane group has keys only or values only
     const int seq = sequence_of(batch, (int)t);
     int64_t pos = 0, at = -1;
     find_row(batch, seq, t, tokens, pages, page_size, kv_heads, pos, at);
-    const int row0 = (int)(unit - t * parts) * rounds * PER + sub;
-    const int row1 = min(row0 + rounds * PER, 2 * kv_heads);
+    const int round0 = (int)(unit - t * parts) * rounds, round1 = round0 + rounds;
+    const int groups = LPR >> group_log;
+    const int64_t base = at + (int64_t)(sub >> 1) * page_size;
+    const uint32_t *codes = (is_v ? v_codes : k_codes) + base * (D / 8) + c;
+    const __half *scales = (is_v ? v_scales : k_scales) + base * groups + (c >> group_log);
+    T *dst = (is_v ? v : k) + (t * kv_heads + (sub >> 1)) * D + 8 * c;
     uint32_t next[kRows];
     __half scale[kRows];
-    auto fetch = [&](int row_) {
+    auto in = [&](int round) { return round < round1 && round * (PER / 2) + (sub >> 1) < kv_heads; };
+    auto fetch = [&](int round) {
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int row = row_ + i * PER;
             next[i] = 0;
             scale[i] = __ushort_as_half(0);
-            if (at >= 0 && row < row1) {
-                const int64_t r = at + (int64_t)(row >> 1) * page_size;
-                next[i] = ((row & 1) ? v_codes : k_codes)[r * (D / 8) + c];
-                scale[i] = ((row & 1) ? v_scales : k_scales)[r * (LPR >> group_log) + (c >> group_log)];
+            if (at >= 0 && in(round + i)) {
+                const int64_t row = (int64_t)((round + i) * (PER / 2)) * page_size;
+                next[i] = codes[row * (D / 8)];
+                scale[i] = scales[row * groups];
             }
         }
     };
-    fetch(row0);
-    for (int row_ = row0; row_ < row1; row_ += kRows * PER) {
+    fetch(round0);
+    for (int round = round0; round < round1 && round * (PER / 2) < kv_heads; round += kRows) {
         uint32_t word[kRows];
-        float s[kRows];
+        __half s[kRows];
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
             word[i] = next[i];
-            s[i] = __half2float(scale[i]);
+            s[i] = scale[i];
         }
-        if (rounds > kRows) fetch(row_ + kRows * PER);
+        fetch(round + kRows);
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            const int row = row_ + i * PER;
-            if (row >= row1) continue;
-            float o[8];
+            if (!in(round + i)) continue;
+            Eight<T> o;
+            values8<T>(word[i], s[i], o.e);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] = (float)nibble_value(word[i] >> (8 * (e >> 1)), e & 1) * s[i];
-            store_row8<T, true>(((row & 1) ? v : k) + ((int64_t)t * kv_heads + (row >> 1)) * D + 8 * c, o);
+            for (int x = 0; x < (int)sizeof(T) / 2; ++x)
+                reinterpret_cast<uint4 *>(dst + (int64_t)((round + i) * (PER / 2)) * D)[x] =
+                    reinterpret_cast<const uint4 *>(o.e)[x];
         }
     }
 }
@@ -504,7 +585,10 @@ int grid_of(int64_t units, int64_t *blocks) {
 template <typename T, bool VEC>
 void rotary_start(const Rows &x, void *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim,
                   const Rotary &rot, int parts, int rounds, unsigned blocks, cudaStream_t st) {
-    auto kern = pairs_of(rot) == kShuffle ? rotary_kernel<T, VEC, kShuffle> : rotary_kernel<T, VEC, kAny>;
+    const int pairs = pairs_of(rot);
+    auto kern = pairs == kShuffle ? rotary_kernel<T, VEC, kShuffle>
+                : pairs == kNext  ? rotary_kernel<T, VEC, kNext>
+                                  : rotary_kernel<T, VEC, kAny>;
     kern<<<blocks, kWarps * 32, 0, st>>>(x, static_cast<T *>(y), y_ts, y_hs, tokens, heads, head_dim, rot, parts,
                                          rounds);
 }
@@ -529,6 +613,7 @@ void append_start(const AppendArgs &a, unsigned blocks, cudaStream_t st) {
     const int pairs = pairs_of(a.rot);
     auto kern = pairs == kNone      ? append_kernel<T, D, VEC, kNone>
                 : pairs == kShuffle ? append_kernel<T, D, VEC, kShuffle>
+                : pairs == kNext    ? append_kernel<T, D, VEC, kNext>
                                     : append_kernel<T, D, VEC, kAny>;
     kern<<<blocks, kWarps * 32, 0, st>>>(a);
 }
@@ -590,6 +675,8 @@ extern "C" int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batc
     if (int rc = check_batch(batch, tokens)) return rc;
     OQ_REQUIRE(k && v, "null pointer argument");
     OQ_REQUIRE(q == nullptr || (q_out != nullptr && q_heads >= 1), "kv4_append: q needs q_out and its head count");
+    OQ_REQUIRE(rotary != nullptr || (q == nullptr && positions == nullptr),
+               "kv4_append: q and positions need a rotary table");
     if (rotary != nullptr)
         if (int rc = check_rotary(rotary, cache->head_dim)) return rc;
     AppendArgs a = {};
