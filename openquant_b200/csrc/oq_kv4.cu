@@ -44,6 +44,7 @@ struct Rotary {
     int dim, flags;
     const void *positions;
     int wide;
+    float one = 1.0f;  // see turn2()
 };
 
 struct Rows {  // [tokens][heads][head_dim] with strides in elements
@@ -99,16 +100,19 @@ __device__ __forceinline__ void load_row8(const T *p, Eight<T> &v) {
 }
 
 template <typename T>
-__device__ __forceinline__ void widen(const Eight<T> &v, float (&x)[8]) {
+__device__ __forceinline__ void widen(const Eight<T> &v, float2 (&x)[4]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Elem<T>::to_f32(v.e[i]);
+    for (int i = 0; i < 4; ++i) x[i] = make_float2(Elem<T>::to_f32(v.e[2 * i]), Elem<T>::to_f32(v.e[2 * i + 1]));
 }
 
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_row8(T *p, const float (&v)[8]) {
+__device__ __forceinline__ void store_row8(T *p, const float2 (&v)[4]) {
     alignas(16) T e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = from_f32<T>(v[i]);
+    for (int i = 0; i < 4; ++i) {
+        e[2 * i] = from_f32<T>(v[i].x);
+        e[2 * i + 1] = from_f32<T>(v[i].y);
+    }
     if (VEC) {
 #pragma unroll
         for (int i = 0; i < (int)sizeof(T) / 2; ++i)
@@ -123,7 +127,7 @@ __device__ __forceinline__ void store_row8(T *p, const float (&v)[8]) {
 // each is multiplied with.  y = x cos + partner * sn, where sn carries the
 // sign of the sum's second term.
 struct Turn {
-    float cs[8], sn[8];
+    float2 cs[4], sn[4];
     bool any;  // one of the eight is rotated
     int src;   // kShuffle: the partners' lane
 };
@@ -143,8 +147,8 @@ __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, T
             for (int q = 0; q < 2; ++q) {
                 const float4 a = __ldg(reinterpret_cast<const float4 *>(row + i0) + q);
                 const float4 b = __ldg(reinterpret_cast<const float4 *>(row + half + i0) + q);
-                t.cs[4 * q] = a.x, t.cs[4 * q + 1] = a.y, t.cs[4 * q + 2] = a.z, t.cs[4 * q + 3] = a.w;
-                t.sn[4 * q] = s * b.x, t.sn[4 * q + 1] = s * b.y, t.sn[4 * q + 2] = s * b.z, t.sn[4 * q + 3] = s * b.w;
+                t.cs[2 * q] = make_float2(a.x, a.y), t.cs[2 * q + 1] = make_float2(a.z, a.w);
+                t.sn[2 * q] = make_float2(s * b.x, s * b.y), t.sn[2 * q + 1] = make_float2(s * b.z, s * b.w);
             }
         }
         return;
@@ -155,9 +159,9 @@ __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, T
             const float4 b = __ldg(reinterpret_cast<const float4 *>(row + half + 4 * c));
             const float cs[4] = {a.x, a.y, a.z, a.w}, sn[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                t.cs[e] = cs[e >> 1];
-                t.sn[e] = ((e & 1) ? sign : -sign) * sn[e >> 1];
+            for (int e = 0; e < 4; ++e) {
+                t.cs[e] = make_float2(cs[e], cs[e]);
+                t.sn[e] = make_float2(-sign * sn[e], sign * sn[e]);
             }
         }
         return;
@@ -166,67 +170,61 @@ __device__ __forceinline__ void load_turn(const Rotary &r, int64_t pos, int c, T
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         const int i = 8 * c + e;
-        t.cs[e] = 1.0f;
-        t.sn[e] = 0.0f;
+        float cs = 1.0f, sn = 0.0f;
         if (i < r.dim) {
             const int a = inter ? i >> 1 : (i < half ? i : i - half);
             const bool first = inter ? !(i & 1) : i < half;
-            t.cs[e] = __ldg(row + a);
-            t.sn[e] = (first ? -sign : sign) * __ldg(row + half + a);
+            cs = __ldg(row + a);
+            sn = (first ? -sign : sign) * __ldg(row + half + a);
         }
+        (e & 1 ? t.cs[e >> 1].y : t.cs[e >> 1].x) = cs;
+        (e & 1 ? t.sn[e >> 1].y : t.sn[e >> 1].x) = sn;
     }
 }
 
-// x cos -+ partner sin with each product and the sum rounded to fp32 (no
-// fused multiply-add): the same bits as the formula in separate operations.
-__device__ __forceinline__ float turn1(float x, float cs, float partner, float sn) {
-    return __fadd_rn(__fmul_rn(x, cs), __fmul_rn(partner, sn));
+// x cos -+ partner sin of two elements, each product and the sum rounded to
+// fp32: the same bits as the formula in separate operations.  The packed
+// multiply and add would be joined into one fused operation even where both
+// are stated as rounding, so the sum is a product with `one` plus the other
+// term: 1.0f from the kernel's arguments, which the compiler does not know.
+__device__ __forceinline__ float2 turn2(float2 x, float2 cs, float2 partner, float2 sn, float one) {
+    return __ffma2_rn(__fmul2_rn(x, cs), make_float2(one, one), __fmul2_rn(partner, sn));
 }
 
 // Rotates a lane's eight elements.  All lanes of the warp take part; `row` is
 // the head's first element (nullptr: no head).
 template <typename T, int PAIRS>
-__device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T *row, int c, float (&x)[8]) {
+__device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T *row, int c, float2 (&x)[4]) {
     if (PAIRS == kShuffle) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float p = __shfl_sync(0xffffffffu, x[e], t.src);
-            if (t.any) x[e] = turn1(x[e], t.cs[e], p, t.sn[e]);
-        }
-        return;
-    }
-    if (PAIRS == kNext) {
-        if (t.any) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                const float a = x[e], b = x[e + 1];
-                x[e] = turn1(a, t.cs[e], b, t.sn[e]);
-                x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
-            }
+        for (int e = 0; e < 4; ++e) {
+            float2 p;
+            p.x = __shfl_sync(0xffffffffu, x[e].x, t.src);
+            p.y = __shfl_sync(0xffffffffu, x[e].y, t.src);
+            if (t.any) x[e] = turn2(x[e], t.cs[e], p, t.sn[e], r.one);
         }
         return;
     }
     if (!t.any) return;
+    if (PAIRS == kNext) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] = turn2(x[e], t.cs[e], make_float2(x[e].y, x[e].x), t.sn[e], r.one);
+        return;
+    }
     const int half = r.dim >> 1;
-    if (r.flags & OQ_ROTARY_INTERLEAVED) {
+    const bool inter = r.flags & OQ_ROTARY_INTERLEAVED;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const float a = x[e], b = x[e + 1];
-            if (8 * c + e < r.dim) {
-                x[e] = turn1(a, t.cs[e], b, t.sn[e]);
-                x[e + 1] = turn1(b, t.cs[e + 1], a, t.sn[e + 1]);
-            }
+    for (int e = 0; e < 4; ++e) {
+        const int i = 8 * c + 2 * e;
+        float2 p = make_float2(x[e].y, x[e].x);
+        if (!inter) {
+            p = make_float2(0.0f, 0.0f);
+            if (row != nullptr && i < r.dim) p.x = Elem<T>::to_f32(row[i < half ? i + half : i - half]);
+            if (row != nullptr && i + 1 < r.dim) p.y = Elem<T>::to_f32(row[i + 1 < half ? i + 1 + half : i + 1 - half]);
         }
-    } else {
-        float p[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int i = 8 * c + e;
-            p[e] = (row != nullptr && i < r.dim) ? Elem<T>::to_f32(row[i < half ? i + half : i - half]) : 0.0f;
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            if (8 * c + e < r.dim) x[e] = turn1(x[e], t.cs[e], p[e], t.sn[e]);
+        const float2 y = turn2(x[e], t.cs[e], p, t.sn[e], r.one);
+        if (i < r.dim) x[e].x = y.x;  // an unrotated element keeps its bits
+        if (i + 1 < r.dim) x[e].y = y.y;
     }
 }
 
@@ -251,35 +249,36 @@ rotary_kernel(Rows x, T *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int head
     const int sub = lane / lpr, c = lane - sub * lpr;
     const int round0 = (int)(unit - t * parts) * rounds;
     const T *xt = static_cast<const T *>(x.p) + t * x.ts;
-    const int last = min((round0 + rounds) * per, heads);  // heads [round0 * per, last)
-    auto row_of = [&](int round) {
-        const int h = round * per + sub;
-        return sub < per && h < last ? xt + h * x.hs : nullptr;
-    };
+    // this lane's heads: every per-th from h on, n of them
+    const int h = round0 * per + sub, end = min((round0 + rounds) * per, heads);
+    const int n = sub < per && h < end ? (end - h + per - 1) / per : 0;
+    const int steps = min(rounds, (heads + per - 1) / per - round0);  // of the warp
+    const T *src = xt + h * x.hs + 8 * c;
+    T *dst = y + t * y_ts + h * y_hs + 8 * c;
+    const int64_t x_step = per * x.hs, y_step = per * y_hs;
     Eight<T> next[kRows];
-    auto fetch = [&](int round) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            if (const T *p = row_of(round + i)) load_row8<T, VEC>(p + 8 * c, next[i]);
-    };
-    fetch(round0);
+    for (int i = 0; i < kRows; ++i)
+        if (i < n) load_row8<T, VEC>(src + i * x_step, next[i]);
     const int64_t pos = position_at(rot, t);
     const bool ok = pos >= 0 && pos < rot.rows;
     if (!ok && lane == 0) index_error();
     Turn turn;
     load_turn<PAIRS>(rot, ok ? pos : 0, c, turn);
-    for (int round = round0; round * per < last; round += kRows) {
-        float v[kRows][8];
+    for (int s = 0; s < steps; s += kRows) {
+        const T *ahead = src + kRows * x_step;
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) widen(next[i], v[i]);
-        if (rounds > kRows) fetch(round + kRows);
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) rotate8<T, PAIRS>(rot, turn, row_of(round + i), c, v[i]);
-        __syncwarp();  // y may be x: partners are read before any store of the warp
-#pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            if (ok && row_of(round + i))
-                store_row8<T, VEC>(y + t * y_ts + ((round + i) * per + sub) * y_hs + 8 * c, v[i]);
+        for (int i = 0; i < kRows; ++i) {
+            if (s + i >= steps) break;
+            float2 v[4];
+            widen(next[i], v);
+            if (s + i + kRows < n) load_row8<T, VEC>(ahead, next[i]);
+            const bool in = s + i < n;
+            rotate8<T, PAIRS>(rot, turn, in ? src - 8 * c : nullptr, c, v);
+            if (PAIRS == kAny) __syncwarp();  // y may be x: partners are read before any store of the warp
+            if (ok && in) store_row8<T, VEC>(dst, v);
+            src += x_step, ahead += x_step, dst += y_step;
+        }
     }
 }
 
@@ -305,14 +304,15 @@ __device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, in
 // fl() the IEEE quotient.  r = x * rcp(s) is within 2e-6 of it where the
 // clipped range is not left, so both round to the same integer unless r is
 // within 1e-5 of a half; then (2 in 10^5), and beyond the range, the word
-// takes the divisions.  Adding 1.5 * 2^23 + 8 leaves u = code + 8 in the low
+// takes the divisions.  (A scale is at least max / 7 (1 - 2^-8), so r leaves
+// [-7.04, 7.04] only where the scale was limited, or is an fp16 subnormal.)
+// Adding 1.5 * 2^23 + 8 leaves u = code + 8 in the low
 // bits of 0x4B400000 + u; the eight sums shifted by 4 e add up, and the
 // constants' own sum is 0x3F400000 (mod 2^32).
 constexpr float kMagic = kRoundMagic + 8.0f;
 
-__device__ __noinline__ uint32_t divide8(float x0, float x1, float x2, float x3, float x4, float x5, float x6, float x7,
-                                         float s) {
-    const float x[8] = {x0, x1, x2, x3, x4, x5, x6, x7};
+__device__ __noinline__ uint32_t divide8(float2 x0, float2 x1, float2 x2, float2 x3, float s) {
+    const float x[8] = {x0.x, x0.y, x1.x, x1.y, x2.x, x2.y, x3.x, x3.y};
     uint32_t acc = 0;
 #pragma unroll
     for (int e = 7; e >= 0; --e)
@@ -320,19 +320,21 @@ __device__ __noinline__ uint32_t divide8(float x0, float x1, float x2, float x3,
     return acc;
 }
 
-__device__ __forceinline__ uint32_t pack8(const float (&x)[8], float s) {
+// mx: the group's largest magnitude.
+__device__ __forceinline__ uint32_t pack8(const float2 (&x)[4], float s, float mx) {
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const float2 inv2 = make_float2(inv, inv), up = make_float2(kMagic, kMagic), down = make_float2(-kMagic, -kMagic);
     uint32_t acc = 0;
-    float off = 0.0f, big = 0.0f;  // the largest distance from an integer, and the largest integer
+    float off = 0.0f;  // the largest distance from an integer
 #pragma unroll
-    for (int e = 7; e >= 0; --e) {
-        const float r = __fmul_rn(x[e], inv), t = __fadd_rn(r, kMagic), n = __fsub_rn(t, kMagic);
-        off = fmaxf(off, fabsf(__fsub_rn(r, n)));
-        big = fmaxf(big, fabsf(n));
-        acc = acc * 16 + __float_as_uint(t);
+    for (int e = 3; e >= 0; --e) {
+        const float2 r = __fmul2_rn(x[e], inv2), t = __fadd2_rn(r, up), n = __fadd2_rn(t, down);
+        const float2 d = __fadd2_rn(r, make_float2(-n.x, -n.y));
+        off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+        acc = (acc * 16 + __float_as_uint(t.y)) * 16 + __float_as_uint(t.x);
     }
-    if (off > 0.49999f || big > 7.0f) acc = divide8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7], s);
+    if (off > 0.49999f || mx > 7.4f * s) acc = divide8(x[0], x[1], x[2], x[3], s);
     return (acc - 0x3F400000u) ^ 0x88888888u;
 }
 
@@ -376,31 +378,28 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
     const int round0 = (int)(unit - t * a.parts) * a.rounds, round1 = min(round0 + a.rounds, a.all_rounds);
 
     // Rounds [round0, q1) are the queries': the lane's head is round * PER +
-    // sub.  Rounds [kv0, kv1) (counted from the first one after the queries)
+    // sub.  Rounds [kv0, ...) (counted from the first one after the queries)
     // are the keys' and values': a lane group has keys only or values only.
-    const int q1 = min(round1, a.q_rounds);
-    const int kv0 = max(round0 - a.q_rounds, 0), kv1 = round1 - a.q_rounds;
+    const int q1 = PAIRS != kNone ? min(round1, a.q_rounds) : 0;
+    const int q_steps = max(q1 - round0, 0), qh = round0 * PER + sub;
+    const int q_n = q_steps > 0 && qh < a.q_heads ? min(q_steps, (a.q_heads - qh + PER - 1) / PER) : 0;
+    const int kv0 = max(round0 - a.q_rounds, 0), kv_steps = max(round1 - a.q_rounds - kv0, 0);
+    const int kvh = kv0 * (PER / 2) + (sub >> 1);
+    const int kv_n = kvh < a.kv_heads ? min(kv_steps, (a.kv_heads - kvh + PER / 2 - 1) / (PER / 2)) : 0;
     const bool is_v = sub & 1;
     const Rows &kv = is_v ? a.v : a.k;
-    const T *q_src = static_cast<const T *>(a.q.p) + t * a.q.ts + sub * a.q.hs + 8 * c;
-    const T *kv_src = static_cast<const T *>(kv.p) + t * kv.ts + (sub >> 1) * kv.hs + 8 * c;
+    const int64_t q_step = PER * a.q.hs, kv_step = (PER / 2) * kv.hs;
+    const T *q_src = static_cast<const T *>(a.q.p) + t * a.q.ts + qh * a.q.hs + 8 * c;
+    const T *kv_src = static_cast<const T *>(kv.p) + t * kv.ts + kvh * kv.hs + 8 * c;
     Eight<T> next[kRows];
-    auto fetch_q = [&](int round) {
 #pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            if (round + i < q1 && (round + i) * PER + sub < a.q_heads)
-                load_row8<T, VEC>(q_src + (int64_t)((round + i) * PER) * a.q.hs, next[i]);
-    };
-    auto fetch_kv = [&](int round) {
-#pragma unroll
-        for (int i = 0; i < kRows; ++i)
-            if (round + i < kv1 && (round + i) * (PER / 2) + (sub >> 1) < a.kv_heads)
-                load_row8<T, VEC>(kv_src + (int64_t)((round + i) * (PER / 2)) * kv.hs, next[i]);
-    };
-    if (round0 < q1)
-        fetch_q(round0);
-    else
-        fetch_kv(kv0);
+    for (int i = 0; i < kRows; ++i) {
+        if (q_steps > 0) {
+            if (i < q_n) load_row8<T, VEC>(q_src + i * q_step, next[i]);
+        } else if (i < kv_n) {
+            load_row8<T, VEC>(kv_src + i * kv_step, next[i]);
+        }
+    }
 
     const int seq = sequence_of(a.batch, (int)t);
     int64_t pos = 0, at = -1;  // place in the sequence; row of head 0 in the cache
@@ -412,66 +411,69 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
     if (PAIRS != kNone) load_turn<PAIRS>(a.rot, ok ? angle : 0, c, turn);
 
     // ---- queries (only with a rotation)
-    if (PAIRS != kNone) {
-        T *dst = static_cast<T *>(a.q_out) + t * a.qo_ts + sub * a.qo_hs + 8 * c;
-        for (int round = round0; round < q1; round += kRows) {
-            float x[kRows][8];
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) widen(next[i], x[i]);
-            if (round + kRows < q1)
-                fetch_q(round + kRows);
-            else
-                fetch_kv(kv0);
+    if (q_steps > 0) {
+        T *dst = static_cast<T *>(a.q_out) + t * a.qo_ts + qh * a.qo_hs + 8 * c;
+        const int64_t out_step = PER * a.qo_hs;
+        for (int s = 0; s < q_steps; s += kRows) {
+            const T *ahead = q_src + kRows * q_step;
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
-                const bool in = round + i < q1 && (round + i) * PER + sub < a.q_heads;
-                rotate8<T, PAIRS>(a.rot, turn, in ? q_src + (int64_t)((round + i) * PER) * a.q.hs - 8 * c : nullptr, c,
-                                  x[i]);
+                if (s + i >= q_steps) break;
+                float2 x[4];
+                widen(next[i], x);
+                if (s + i + kRows < q_n) load_row8<T, VEC>(ahead, next[i]);
+                const bool in = s + i < q_n;
+                rotate8<T, PAIRS>(a.rot, turn, in ? q_src - 8 * c : nullptr, c, x);
+                if (PAIRS == kAny) __syncwarp();  // q_out may be q: partners are read before any store of the warp
+                if (ok && in) store_row8<T, VEC>(dst, x);
+                q_src += q_step, ahead += q_step, dst += out_step;
             }
-            __syncwarp();  // q_out may be q: partners are read before any store of the warp
-#pragma unroll
-            for (int i = 0; i < kRows; ++i)
-                if (ok && round + i < q1 && (round + i) * PER + sub < a.q_heads)
-                    store_row8<T, VEC>(dst + (int64_t)((round + i) * PER) * a.qo_hs, x[i]);
         }
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+            if (i < kv_n) load_row8<T, VEC>(kv_src + i * kv_step, next[i]);
     }
 
     // ---- keys and values
     if (PAIRS != kNone) turn.any = turn.any && !is_v;
     const unsigned pair = (LPR == 16 ? 0xffffffffu : 0xffffu) << ((sub >> 1) * 2 * LPR % 32);
-    const int lanes = 1 << a.group_log, groups = LPR >> a.group_log;
-    const bool first = (c & (lanes - 1)) == 0;
-    uint32_t *codes = (is_v ? a.v_codes : a.k_codes) + (at + (int64_t)(sub >> 1) * a.page_size) * (D / 8) + c;
-    __half *scales = (is_v ? a.v_scales : a.k_scales) + (at + (int64_t)(sub >> 1) * a.page_size) * groups +
-                     (c >> a.group_log);
-    for (int round = kv0; round < kv1; round += kRows) {
-        float x[kRows][8];
-#pragma unroll
-        for (int i = 0; i < kRows; ++i) widen(next[i], x[i]);
-        fetch_kv(round + kRows);
+    const int groups = LPR >> a.group_log;
+    const bool put = at >= 0 && ok, first = put && (c & ((1 << a.group_log) - 1)) == 0;
+    const int64_t row = at + (int64_t)kvh * a.page_size;
+    uint32_t *codes = (is_v ? a.v_codes : a.k_codes) + row * (D / 8) + c;
+    __half *scales = (is_v ? a.v_scales : a.k_scales) + row * groups + (c >> a.group_log);
+    const int64_t code_step = (int64_t)(PER / 2) * a.page_size * (D / 8);
+    const int64_t scale_step = (int64_t)(PER / 2) * a.page_size * groups;
+    for (int s = 0; s < kv_steps; s += kRows) {
+        const T *ahead = kv_src + kRows * kv_step;
 #pragma unroll
         for (int i = 0; i < kRows; ++i) {
-            if (round + i >= kv1) break;  // warp-uniform
-            const int head = (round + i) * (PER / 2) + (sub >> 1);
-            const bool in = head < a.kv_heads;
-            if (PAIRS != kNone)
-                rotate8<T, PAIRS>(a.rot, turn,
-                                  in ? kv_src + (int64_t)((round + i) * (PER / 2)) * kv.hs - 8 * c : nullptr, c, x[i]);
-            // the largest magnitude as its bits: an infinity or a NaN is at least 0x7F800000
-            uint32_t mx = 0;
+            if (s + i >= kv_steps) break;  // warp-uniform
+            float2 x[4];
+            widen(next[i], x);
+            if (s + i + kRows < kv_n) load_row8<T, VEC>(ahead, next[i]);
+            const bool in = s + i < kv_n;
+            if (PAIRS != kNone) rotate8<T, PAIRS>(a.rot, turn, in ? kv_src - 8 * c : nullptr, c, x);
+            float mx = 0.0f;
+            float2 nan = make_float2(0.0f, 0.0f);  // 0 * x: NaN where x is not finite
 #pragma unroll
-            for (int e = 0; e < 8; ++e) mx = max(mx, __float_as_uint(x[i][e]) & 0x7FFFFFFFu);
+            for (int e = 0; e < 4; ++e) {
+                mx = fmaxf(mx, fmaxf(fabsf(x[e].x), fabsf(x[e].y)));
+                nan = __ffma2_rn(x[e], make_float2(0.0f, 0.0f), nan);
+            }
             // Not finite anywhere in the token's key or value of this head: the
             // lanes of both (2 * LPR of them) agree on it.
-            const bool bad = (__ballot_sync(0xffffffffu, in && mx >= 0x7F800000u) & pair) != 0;
-            for (int o = 0; o < a.group_log; ++o) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1 << o));
-            const float s = bad ? 1.0f : scale_of(__uint_as_float(mx));
-            const uint32_t word = bad ? 0u : pack8(x[i], s);
-            if (in && at >= 0 && ok) {
-                const int64_t row = (int64_t)((round + i) * (PER / 2)) * a.page_size;
-                codes[row * (D / 8)] = word;
-                if (first) scales[row * groups] = bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(s);
-            }
+            const bool bad = (__ballot_sync(0xffffffffu, in && !(nan.x + nan.y == 0.0f)) & pair) != 0;
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+            if (a.group_log > 2) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            if (a.group_log > 3) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            const float sc = bad ? 1.0f : scale_of(mx);
+            uint32_t word = pack8(x, sc, bad ? 0.0f : mx);
+            if (bad) word = 0;
+            if (put && in) *codes = word;
+            if (first && in) *scales = bad && !is_v ? __ushort_as_half(0x7FFF) : __float2half_rn(sc);
+            kv_src += kv_step, ahead += kv_step, codes += code_step, scales += scale_step;
         }
     }
 }
@@ -557,14 +559,15 @@ read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_c
 }
 
 // Rounds a warp takes of a token that has `all`: as many as leave the GPU
-// kFill warps a SM, in steps of kRows.  (Few: a warp's lookups are paid for
-// more often; many: too few warps at small sizes.)
-constexpr int kFill = 32;
+// kFill warps a SM, in steps of kRows, at most kMost.  (Few: a warp's lookups
+// are paid for more often; many: too few warps at small sizes, and a last
+// wave of warps that leaves SMs idle.)
+constexpr int kFill = 32, kMost = 16;
 
 int rounds_of(int64_t tokens, int64_t all) {
     const int64_t want = tokens * all / ((int64_t)sm_count() * kFill);
     const int64_t r = want / kRows * kRows;
-    return (int)(r < kRows ? kRows : (r > all ? cdiv(all, kRows) * kRows : r));
+    return (int)(r < kRows ? kRows : (r > kMost ? kMost : r));
 }
 
 int check_rotary(const oq_rotary_spec *r, int head_dim) {

@@ -146,6 +146,11 @@ def _heads(x, name, dtypes=(torch.float16, torch.bfloat16)):
     return tokens, heads, dim
 
 
+def _like(x):
+    """A contiguous tensor like x (empty_like, the quicker call, keeps strides)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _call(dev, fn, *args):
     """fn(*args, stream) on the tensors' GPU, its status checked."""
     if torch.cuda.current_device() == dev:
@@ -178,7 +183,7 @@ def rotary(x, table, positions, *, interleaved=False, inverse=False, out=None):
                         dev)
     pos, wide = _positions(positions, tokens, dev)
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+        out = _like(x)
     elif (out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != dev
           or (out.stride(2) != 1 and dim > 1)):
         raise ValueError("out must be like x, with contiguous heads")
@@ -369,7 +374,7 @@ class Int4KVCache:
             if qt != tokens or qd != dim or q.dtype is not k.dtype or q.get_device() != dev:
                 raise ValueError("q must have k's tokens, head_dim, dtype and GPU")
             if q_out is None:
-                q_out = torch.empty((qt, qh, qd), dtype=q.dtype, device=self._device)
+                q_out = _like(q)
             elif (q_out.shape != q.shape or q_out.dtype is not q.dtype or q_out.get_device() != dev
                   or q_out.stride(2) != 1):
                 raise ValueError("q_out must be like q, with contiguous heads")
@@ -395,9 +400,7 @@ class Int4KVCache:
         if dtype not in _CODES:
             raise ValueError("dtype must be torch.float16, torch.bfloat16 or torch.float32")
         self._check_batch(batch, self._dev)
-        shape = (tokens, self.kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=dtype, device=self._device)
-        v = torch.empty(shape, dtype=dtype, device=self._device)
+        k, v = torch.empty((2, tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self._device).unbind(0)
         _call(self._dev, self._lib.oq_kv4_read, self._ref, batch._ref, k.data_ptr(), v.data_ptr(), _CODES[dtype],
               tokens)
         return k, v
@@ -428,7 +431,7 @@ class Int4KVCache:
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
         if out is None:
-            out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=self._device)
+            out = _like(q)
         elif (out.shape != q.shape or out.dtype is not q.dtype or out.get_device() != dev
               or not out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor like q")
