@@ -368,7 +368,7 @@ struct AppendArgs {
 };
 
 template <typename T, int D, bool VEC, int PAIRS>
-__global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_constant__ AppendArgs a) {
+__global__ void __launch_bounds__(kWarps * 32, VEC && PAIRS != kAny ? 6 : 1) append_kernel(const __grid_constant__ AppendArgs a) {
     constexpr int LPR = D / 8, PER = 32 / LPR;
     const int lane = threadIdx.x & 31;
     const int64_t unit = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
@@ -559,15 +559,17 @@ read_kernel(const uint32_t *k_codes, const __half *k_scales, const uint32_t *v_c
 }
 
 // Rounds a warp takes of a token that has `all`: as many as leave the GPU
-// kFill warps a SM, in steps of kRows, at most kMost.  (Few: a warp's lookups
+// kFill warps a SM, in steps of kRows, at most `most`.  (Few: a warp's lookups
 // are paid for more often; many: too few warps at small sizes, and a last
-// wave of warps that leaves SMs idle.)
-constexpr int kFill = 32, kMost = 16;
+// wave of warps that leaves SMs idle.  Measured, 8 to 48 rounds: rotary of
+// 8192 x 64 x 128 50 to 45 us, least at 16; append and read of 7622 tokens of
+// 32 heads 158 to 136 us, flat from 24 on, where the lookups are a longer chain.)
+constexpr int kFill = 32;
 
-int rounds_of(int64_t tokens, int64_t all) {
+int rounds_of(int64_t tokens, int64_t all, int most) {
     const int64_t want = tokens * all / ((int64_t)sm_count() * kFill);
     const int64_t r = want / kRows * kRows;
-    return (int)(r < kRows ? kRows : (r > kMost ? kMost : r));
+    return (int)(r < kRows ? kRows : (r > most ? most : r));
 }
 
 int check_rotary(const oq_rotary_spec *r, int head_dim) {
@@ -600,7 +602,7 @@ template <typename T>
 int rotary_launch(const Rows &x, void *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim,
                   const Rotary &rot, cudaStream_t st) {
     const int64_t all = cdiv(heads, 32 / (head_dim / 8));
-    const int rounds = rounds_of(tokens, all), parts = (int)cdiv(all, rounds);
+    const int rounds = rounds_of(tokens, all, 16), parts = (int)cdiv(all, rounds);
     int64_t blocks;
     if (int rc = grid_of(tokens * parts, &blocks)) return rc;
     const int64_t n = 16 / sizeof(T);
@@ -702,7 +704,7 @@ extern "C" int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batc
     const int per = 32 / (cache->head_dim / 8);
     a.q_rounds = (int)cdiv(a.q_heads, per);
     a.all_rounds = a.q_rounds + (int)cdiv(2 * a.kv_heads, per);
-    a.rounds = rounds_of(tokens, a.all_rounds);
+    a.rounds = rounds_of(tokens, a.all_rounds, 32);
     a.parts = (int)cdiv(a.all_rounds, a.rounds);
     if (rotary != nullptr)
         a.rot = Rotary{rotary->table, rotary->rows, rotary->dim, rotary->flags, positions, positions_64};
@@ -731,7 +733,7 @@ extern "C" int oq_kv4_read(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
     OQ_REQUIRE(aligned(k, 16) && aligned(v, 16), "kv4_read: k and v must be 16-byte aligned");
     const int per = 32 / (cache->head_dim / 8);
     const int64_t all = cdiv(2 * cache->kv_heads, per);
-    const int rounds = rounds_of(tokens, all), parts = (int)cdiv(all, rounds);
+    const int rounds = rounds_of(tokens, all, 32), parts = (int)cdiv(all, rounds);
     int64_t blocks;
     if (int rc = grid_of(tokens * parts, &blocks)) return rc;
     const int gl = group_log_of(cache->group_size);
