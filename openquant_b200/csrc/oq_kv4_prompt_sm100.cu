@@ -4,7 +4,7 @@
 // Mathematics.  A CTA has 256 query rows of one key head -- rows are (token,
 // query head of the key head) in that order, so all query heads that share a
 // key head share its dequantization -- as two tiles of 128, and walks the
-// cache in blocks of 128 tokens:
+// cache in blocks of 64 tokens:
 //     S = Q K^T (fp32 in TMEM),  p = 2^(S f - m),  O = O + P V
 // with the running maximum m of a row raised only when a score passes it by
 // 2^14 (see kRaise): then O, in TMEM, is multiplied by 2^(m_old - m_new);
@@ -15,8 +15,9 @@
 //
 // Roles: warps 0-3 and 4-7 are the softmax of the two tiles (a thread a row),
 // warps 8-11 turn codes into fp16 tiles, one thread of warp 12 issues the
-// products.  While one tile's softmax runs, the other tile's products do:
-// the issue order is P0 V, Q0 K', P1 V, Q1 K', ...
+// products.  Each tile has two S buffers: the scores of a block are computed
+// two blocks ahead of its P V, so a softmax warp finds its next scores ready
+// and the products run while it works.
 //
 // Layouts: Q and K tiles are K-major, 128-byte swizzled, 64 elements a panel;
 // V tiles have the same bytes (row = token) read as an MN-major operand.
@@ -30,17 +31,23 @@ namespace kv4 {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTok = 128;  // cached tokens of a block
+constexpr int kTok = 128;   // cached tokens of a block
+constexpr int kStages = 2;  // K and V tiles in shared memory
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kS = 0, kO = 256;  // TMEM columns: S tiles at 0 and 128, O tiles at 256 and 256 + head_dim
-constexpr int kSoftmaxRegs = 184, kDequantRegs = 104, kIssueRegs = 40;
-static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * (65536 / kThreads), "register split");
+// TMEM columns: S buffers (tile, block & 1) of kTok at 0, O tiles at 256 and 256 + head_dim
+constexpr uint32_t kS = 0, kO = 256;
+// Registers a thread: all warps start with kLaunchRegs; the dequantizing and
+// the issuing warpgroup give some up (dec, never above what they have), the
+// softmax warpgroups take them (inc, never below).
+constexpr int kLaunchRegs = 65536 / kThreads, kSoftmaxRegs = 192, kDequantRegs = 88, kIssueRegs = 40;
+static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * kLaunchRegs, "register split");
+static_assert(kSoftmaxRegs >= kLaunchRegs && kDequantRegs <= kLaunchRegs && kIssueRegs <= kLaunchRegs, "");
 
 template <int HD>
 struct Smem {
-    static constexpr int kPanel = kTok * 128;          // 64 elements of 128 rows
-    static constexpr int kTile = kPanel * (HD / 64);   // Q, K or V tile
-    static constexpr int kQ = 0, kK = 2 * kTile, kV = 4 * kTile, kBars = 6 * kTile;
+    static constexpr int kQPanel = 128 * 128, kPanel = kTok * 128;  // 64 elements of every row
+    static constexpr int kQTile = kQPanel * (HD / 64), kTile = kPanel * (HD / 64);
+    static constexpr int kQ = 0, kK = 2 * kQTile, kV = kK + kStages * kTile, kBars = kV + kStages * kTile;
     static constexpr int kBytes = kBars + 256 + 1024;  // barriers; slack to align to 1024
 };
 
@@ -49,6 +56,12 @@ struct Smem {
 __device__ __forceinline__ uint64_t desc_mn_sw128(uint32_t addr, int panel) {
     return (uint64_t)((addr & 0x3FFFF) >> 4) | (uint64_t)(panel >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
            (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+__device__ __forceinline__ void tmem_ld_32x32b_x8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr));
 }
 
 template <int R>
@@ -60,12 +73,20 @@ __device__ __forceinline__ void regs_dec() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(R));
 }
 
+// One lane of a converged warp, in a form in which the compiler knows that the
+// warp is converged: it then keeps the products' operands in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t v;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(v));
+    return v != 0;
+}
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Byte offset of the 16-byte chunk `c` (eight elements) of row r.
-template <int HD>
+template <int PANEL>
 __device__ __forceinline__ uint32_t chunk_at(int r, int c) {
-    return (uint32_t)((c >> 3) * Smem<HD>::kPanel + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+    return (uint32_t)((c >> 3) * PANEL + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -79,10 +100,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
-    uint64_t *q_full = bars, *s_full = bars + 2, *p_full = bars + 4, *k_full = bars + 6, *k_empty = bars + 8,
-             *v_full = bars + 10, *v_empty = bars + 12, *done = bars + 14;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(bars + 16);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // s_full, p_full: [tile][block & 1]; pv_done: [tile]
+    uint64_t *q_full = bars, *done = bars + 1, *pv_done = bars + 2, *s_full = bars + 4, *p_full = bars + 8,
+             *k_full = bars + 12, *k_empty = k_full + kStages, *v_full = k_empty + kStages,
+             *v_empty = v_full + kStages;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_empty + kStages);
+    static_assert((12 + 4 * kStages) * 8 + 4 <= 256, "barrier space");
+    const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     // ---- this CTA's item: items before each sequence, then the sequence
     __shared__ int warp_sum[kThreads / 32], found[2];
@@ -138,10 +162,14 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     const int tiles = nrows > 128 ? 2 : 1;
 
     if (tid == 0) {
-        mbar_init(&q_full[0], 128 * tiles);
-        for (int i = 0; i < 2; ++i) {
+        mbar_init(q_full, 128 * tiles);
+        for (int i = 0; i < 4; ++i) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 128);
+        }
+        mbar_init(&pv_done[0], 1);
+        mbar_init(&pv_done[1], 1);
+        for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], 128);
             mbar_init(&v_full[i], 128);
             mbar_init(&k_empty[i], 1);
@@ -183,7 +211,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 float up = fp16_power<T>(top, down);
                 f *= down;
                 if (a.f < 0.0f) up = -up;
-                const uint32_t dst = smem_u32(smem + L::kQ + wg * L::kTile);
+                const uint32_t dst = smem_u32(smem + L::kQ + wg * L::kQTile);
                 for (int c = 0; c < HD / 8; ++c) {
                     uint32_t w[4] = {0, 0, 0, 0};
                     if (in) {
@@ -191,10 +219,10 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
                         for (int e = 0; e < 4; ++e) w[e] = as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up));
                     }
-                    st16(dst + chunk_at<HD>(r, c), w[0], w[1], w[2], w[3]);
+                    st16(dst + chunk_at<L::kQPanel>(r, c), w[0], w[1], w[2], w[3]);
                 }
                 fence_async_smem();
-                mbar_arrive(&q_full[0]);
+                mbar_arrive(q_full);
             }
             if (f == 0.0f) f = 1e-30f;  // masked scores are -inf before they are multiplied
             const int64_t pos = base + tk;
@@ -204,8 +232,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int64_t all_vis = a.causal ? base + (row0 + wg * 128) / a.ratio + 1 : length;
             const int64_t all_low = a.window > 0 ? base + last / a.ratio + 1 - a.window : 0;
             const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-            const uint32_t ts = tmem + quarter + kS + wg * 128, to = tmem + quarter + kO + wg * HD;
-            float m = -1e30f, l = 0.0f;
+            const uint32_t ts = tmem + quarter + kS + wg * kTok, to = tmem + quarter + kO + wg * HD;
+            float m = -1e30f;
+            float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             bool ok = true;
             for (int j = 0; j < nblk; ++j) {
                 ok = __all_sync(0xffffffffu, mbar_wait(&s_full[wg], j & 1));
@@ -220,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     const int e0 = (int)min(max(low - t0, (int64_t)0), (int64_t)kTok);
                     const int e1 = (int)min(max(vis - t0, (int64_t)0), (int64_t)kTok);
 #pragma unroll
-                    for (int i = 0; i < 128; ++i)
+                    for (int i = 0; i < kTok; ++i)
                         if (i < e0 || i >= e1) s[i >> 5][i & 31] = 0xff800000u;
                 }
                 float mx[4];
@@ -228,46 +257,51 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 for (int i = 0; i < 4; ++i) {
                     mx[i] = __uint_as_float(s[i][0]);
 #pragma unroll
-                    for (int e = 1; e < 32; ++e) mx[i] = fmaxf(mx[i], __uint_as_float(s[i][e]));
+                    for (int e = 1; e < 31; e += 2)
+                        mx[i] = fmaxf(fmaxf(mx[i], __uint_as_float(s[i][e])), __uint_as_float(s[i][e + 1]));
+                    mx[i] = fmaxf(mx[i], __uint_as_float(s[i][31]));
                 }
                 const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
                 const bool raise = top > m + kRaise;
                 if (__any_sync(0xffffffffu, raise)) {
                     const float mn = raise ? top - kLift : m, corr = ex2(m - mn);
-                    l *= corr;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) l2[i].x *= corr, l2[i].y *= corr;
                     m = mn;
                     if (j > 0) {  // P V of the block before is complete: it was issued before this S
-#pragma unroll
-                        for (int i = 0; i < HD / 32; ++i) {
-                            uint32_t o[32];
-                            tmem_ld_32x32b_x32(to + 32 * i, o);
+#pragma unroll 1
+                        for (int i = 0; i < HD / 8; ++i) {
+                            uint32_t o[8];
+                            tmem_ld_32x32b_x8(to + 8 * i, o);
                             tc_wait_ld();
 #pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
-                            tmem_st_32x32b_x32(to + 32 * i, o);
+                            for (int e = 0; e < 8; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * corr);
+                            tmem_st_32x32b_x8(to + 8 * i, o);
                         }
                     }
                 }
-                float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const float2 f2 = make_float2(f, f), m2 = make_float2(-m, -m);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    uint32_t p[32];
+                for (int h = 0; h < 4; ++h) {
+                    uint32_t p[16];
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int c = 64 * i + 2 * e;
-                        const float x = ex2(fmaf(__uint_as_float(s[c >> 5][c & 31]), f, -m));
-                        const float y = ex2(fmaf(__uint_as_float(s[(c + 1) >> 5][(c + 1) & 31]), f, -m));
-                        sum[e & 1] += x;
-                        sum[2 + (e & 1)] += y;
-                        p[e] = as_u32(__floats2half2_rn(x, y));
+                    for (int e = 0; e < 16; ++e) {
+                        float2 x = __ffma2_rn(make_float2(__uint_as_float(s[h][2 * e]), __uint_as_float(s[h][2 * e + 1])),
+                                              f2, m2);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        l2[e & 1] = __fadd2_rn(l2[e & 1], x);
+                        p[e] = as_u32(__floats2half2_rn(x.x, x.y));
                     }
-                    tmem_st_32x32b_x32(ts + 32 * i, p);
+                    tmem_st_32x32b_x16(ts + 16 * h, p);
+                    if (h & 1) {  // half of P is ready: it is multiplied while the other half is made
+                        tc_wait_st();
+                        tc_fence_before();
+                        mbar_arrive(&p_full[2 * wg + (h >> 1)]);
+                    }
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                tc_wait_st();
-                tc_fence_before();
-                mbar_arrive(&p_full[wg]);
             }
+            const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
             // ------------------------------------------------- epilogue
             if (nblk > 0) {
                 ok = __all_sync(0xffffffffu, ok && mbar_wait(done, 0));
@@ -301,48 +335,54 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     a.log_sum[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
             }
         }
-    } else if (warp < 12) {
+        tc_fence_before();
+        __syncthreads();
+        return;  // each role ends by itself: the compiler then knows its register count
+    }
+    if (warp < 12) {
         // ---------------------------------------------------- dequantize
         regs_dec<kDequantRegs>();
-        constexpr int N = HD / 32;  // 16-byte chunks of codes a thread takes of a K or V block
+        constexpr int N = kTok * CH / 128;  // 16-byte chunks of codes a thread takes of a K or V block
+        constexpr int B16 = kTok / 16, kAhead = 32 / B16;  // 16-token rows of a block; blocks of one look-up
         const int r = tid & 127;
         const int per = a.page_size >> 4;
-        uint32_t row16 = 0;  // lane i < 8: row / 16 in the cache of the block's i-th 16 tokens
+        uint32_t row16 = 0;  // lane i: row / 16 in the cache of 16 tokens, from block `j` on
         auto look_up = [&](int j) {
-            uint32_t v = 0;
+            row16 = 0;
             const int64_t t = lo + (int64_t)j * kTok + lane * 16;
-            if (lane < 8 && t < hi && t + 16 > floor) {
+            if (t < hi && t + 16 > floor) {
                 const int blk = (int)(t >> 4), pg = blk / per;
                 const int page = __ldg(a.batch.table + (int64_t)b * a.batch.max_pages + pg);
                 if (page < 0 || page >= a.pages)
                     index_error();
                 else
-                    v = (uint32_t)(((int64_t)page * a.kv_heads + head) * per + (blk - pg * per));
+                    row16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * per + (blk - pg * per));
             }
-            return v;
         };
         uint4 kc[N], vc[N];
         uint32_t sc[N];  // scales of a chunk: K low, V high half
         // chunk i of the thread: token (r + 128 i) / CH, 16-byte chunk (r + 128 i) % CH
         auto load = [&](int j, bool keys) {
+            if (j >= nblk) return;
+            if (keys && j % kAhead == 0) look_up(j);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int id = r + 128 * i, tk = id / CH, c = id % CH;
-                const uint32_t r16 = __shfl_sync(0xffffffffu, row16, tk >> 4);
+                const uint32_t r16 = __shfl_sync(0xffffffffu, row16, (j % kAhead) * B16 + (tk >> 4));
                 const size_t row = (size_t)r16 * 16 + (tk & 15);
                 const int64_t t = lo + (int64_t)j * kTok + tk;
+                const uint4 w = __ldg(reinterpret_cast<const uint4 *>((keys ? a.k_codes : a.v_codes) + row * (HD / 2) +
+                                                                      c * 16));
                 // tokens that no row of the block sees may be anything: they become 0
-                const bool live = t < hi && t >= floor;
-                const uint8_t *codes = (keys ? a.k_codes : a.v_codes) + row * (HD / 2) + c * 16;
-                const __half *scale = (keys ? a.k_scales : a.v_scales) + row * NG + c * 32 / GS;
-                const uint4 w = __ldg(reinterpret_cast<const uint4 *>(codes));
-                const uint32_t s = live ? (uint32_t)__half_as_ushort(__ldg(scale)) : 0u;
+                const uint32_t x = t < hi && t >= floor ? (uint32_t)__half_as_ushort(__ldg(
+                                                              (keys ? a.k_scales : a.v_scales) + row * NG + c * 32 / GS))
+                                                        : 0u;
                 if (keys) {
                     kc[i] = w;
-                    sc[i] = (sc[i] & 0xffff0000u) | s;
+                    sc[i] = (sc[i] & 0xffff0000u) | x;
                 } else {
                     vc[i] = w;
-                    sc[i] = (sc[i] & 0xffffu) | s << 16;
+                    sc[i] = (sc[i] & 0xffffu) | x << 16;
                 }
             }
         };
@@ -367,91 +407,100 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     unpack_int(word[x], v);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = __hmul2(v[e], s2);
-                    st16(dst + chunk_at<HD>(tk, 4 * c + (x ^ (swap ? 2 : 0))), as_u32(v[0]), as_u32(v[1]), as_u32(v[2]),
-                         as_u32(v[3]));
+                    st16(dst + chunk_at<L::kPanel>(tk, 4 * c + (x ^ (swap ? 2 : 0))), as_u32(v[0]), as_u32(v[1]),
+                         as_u32(v[2]), as_u32(v[3]));
                 }
             }
         };
-        if (nblk > 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) sc[i] = 0;
-            row16 = look_up(0);
-            load(0, true);
-            load(0, false);
-            row16 = look_up(1);
-        }
+        for (int i = 0; i < N; ++i) sc[i] = 0;
+        load(0, true);
+        load(0, false);
         bool ok = true;
-        for (int j = 0; j < nblk; ++j) {
-            const int st = j & 1;
-            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], ((j >> 1) - 1) & 1));
+        for (int j = 0; ok && j < nblk; ++j) {
+            const int st = j % kStages, turn = j / kStages;
+            if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (turn - 1) & 1));
             if (!ok) break;
             store(smem_u32(smem + L::kK + st * L::kTile), kc, true);
             fence_async_smem();
             mbar_arrive(&k_full[st]);
-            if (j + 1 < nblk) load(j + 1, true);
-            if (j >= 2) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], ((j >> 1) - 1) & 1));
+            load(j + 1, true);
+            if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], (turn - 1) & 1));
             if (!ok) break;
             store(smem_u32(smem + L::kV + st * L::kTile), vc, false);
             fence_async_smem();
             mbar_arrive(&v_full[st]);
-            if (j + 1 < nblk) load(j + 1, false);
-            row16 = look_up(j + 2);
+            load(j + 1, false);
         }
-    } else {
+        tc_fence_before();
+        __syncthreads();
+        return;
+    }
+    {
         // --------------------------------------------------------- issue
         regs_dec<kIssueRegs>();
-        if (warp == 12 && lane == 0 && nblk > 0) {
+        const int blocks_u = __shfl_sync(0xffffffffu, nblk, 0), tiles_u = __shfl_sync(0xffffffffu, tiles, 0);
+        const uint32_t tmem_u = __shfl_sync(0xffffffffu, tmem, 0);
+        if (warp == 12 && blocks_u > 0) {  // the whole warp walks, one lane issues
             constexpr uint32_t id_qk = umma_idesc_f16(128, kTok, false);
             constexpr uint32_t id_pv = umma_idesc_f16(128, HD, false) | 1u << 16;  // B is MN-major
             const uint32_t q0 = smem_u32(smem + L::kQ);
             auto scores = [&](int i, int j) {
-                const uint64_t qd = umma_desc_sw128(q0 + i * L::kTile);
-                const uint64_t kd = umma_desc_sw128(smem_u32(smem + L::kK + (j & 1) * L::kTile));
+                const uint64_t qd = umma_desc_sw128(q0 + i * L::kQTile);
+                const uint64_t kd = umma_desc_sw128(smem_u32(smem + L::kK + (j % kStages) * L::kTile));
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) {
-                    const uint64_t off = (uint64_t)((k >> 2) * L::kPanel + (k & 3) * 32) >> 4;
-                    tc_mma_ss(tmem + kS + i * 128, qd + off, kd + off, id_qk, k != 0);
+                    for (int k = 0; k < HD / 16; ++k)
+                        tc_mma_ss(tmem_u + kS + i * kTok, qd + ((uint64_t)((k >> 2) * L::kQPanel + (k & 3) * 32) >> 4),
+                                  kd + ((uint64_t)((k >> 2) * L::kPanel + (k & 3) * 32) >> 4), id_qk, k != 0);
+                    tc_commit(&s_full[i]);
+                    if (i == tiles_u - 1) tc_commit(&k_empty[j % kStages]);
                 }
-                tc_commit(&s_full[i]);
+                __syncwarp();
             };
-            auto values = [&](int i, int j) {
-                const uint64_t vd = desc_mn_sw128(smem_u32(smem + L::kV + (j & 1) * L::kTile), L::kPanel);
+            auto values = [&](int i, int j, int h) {
+                const uint64_t vd = desc_mn_sw128(smem_u32(smem + L::kV + (j % kStages) * L::kTile), L::kPanel);
+                if (elect_one()) {
 #pragma unroll
-                for (int k = 0; k < kTok / 16; ++k)
-                    tc_mma_ts(tmem + kO + i * HD, tmem + kS + i * 128 + k * 8, vd + (uint64_t)(k * 16 * 128 >> 4),
-                              id_pv, j != 0 || k != 0);
+                    for (int k = 4 * h; k < 4 * h + 4; ++k)
+                        tc_mma_ts(tmem_u + kO + i * HD, tmem_u + kS + i * kTok + k * 8,
+                                  vd + (uint64_t)(k * 16 * 128 >> 4), id_pv, j != 0 || k != 0);
+                    if (h == 1 && i == tiles_u - 1) tc_commit(&v_empty[j % kStages]);
+                }
+                __syncwarp();
             };
-            bool ok = mbar_wait(&q_full[0], 0) && mbar_wait(&k_full[0], 0);
+            bool ok = mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0);
             if (ok) {
                 tc_fence_after();
-                for (int i = 0; i < tiles; ++i) scores(i, 0);
-                tc_commit(&k_empty[0]);
+                for (int i = 0; i < tiles_u; ++i) scores(i, 0);
             }
-            for (int j = 0; ok && j < nblk; ++j) {
-                if (!(ok = mbar_wait(&v_full[j & 1], (j >> 1) & 1))) break;
-                for (int i = 0; i < tiles; ++i) {
-                    if (!(ok = mbar_wait(&p_full[i], j & 1))) break;
+            for (int j = 0; ok && j < blocks_u; ++j) {
+                if (!(ok = mbar_wait(&v_full[j % kStages], (j / kStages) & 1))) break;
+                for (int i = 0; i < tiles_u; ++i) {
+                    if (!(ok = mbar_wait(&p_full[2 * i], j & 1))) break;
                     tc_fence_after();
-                    values(i, j);
-                    if (i == tiles - 1) tc_commit(&v_empty[j & 1]);
-                    if (j + 1 < nblk) {
-                        if (i == 0 && !(ok = mbar_wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1))) break;
+                    values(i, j, 0);
+                    if (!(ok = mbar_wait(&p_full[2 * i + 1], j & 1))) break;
+                    tc_fence_after();
+                    values(i, j, 1);
+                    if (j + 1 < blocks_u) {
+                        if (i == 0 && !(ok = mbar_wait(&k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1))) break;
                         tc_fence_after();
                         scores(i, j + 1);
-                        if (i == tiles - 1) tc_commit(&k_empty[(j + 1) & 1]);
                     }
                 }
             }
             // Every product this thread issued has completed once `done` fires.
-            tc_commit(done);
+            if (elect_one()) tc_commit(done);
+            __syncwarp();
             mbar_wait(done, 0);
         }
         __syncwarp();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+        if (warp == 12) tmem_dealloc(tmem, kTmemCols);
     }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    if (warp == 12) tmem_dealloc(tmem, kTmemCols);
 }
 
 template <typename T, int HD, int GS>
