@@ -533,7 +533,7 @@ OQ_API int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *batch
                             oq_stream_t stream);
 OQ_API int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache,
                                                 const oq_kv4_batch *batch,
-                                                int q_heads);
+                                                int q_heads, int64_t tokens);
 
 #ifdef __cplusplus
 }

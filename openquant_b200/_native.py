@@ -55,7 +55,7 @@ SIGNATURES = {
     "oq_kv4_read": (_I32, [_P, _P, _P, _P, _I32, _I64, _P]),
     "oq_kv4_attention": (_I32, [_P, _P, _P, _I32, _I32, _I64, _I64, _P, _P, _I64, ctypes.c_float, _I64, _I32, _P,
                                 ctypes.c_size_t, _P]),
-    "oq_kv4_attention_workspace_bytes": (_I64, [_P, _P, _I32]),
+    "oq_kv4_attention_workspace_bytes": (_I64, [_P, _P, _I32, _I64]),
     "oq_peer_alloc": (_I32, [ctypes.c_size_t, _P]),
     "oq_peer_free": (_I32, [_P]),
     "oq_peer_export": (_I32, [_P, _P]),

@@ -707,6 +707,20 @@ int attention_typed(Args &a, const oq_kv4_cache *c, const oq_kv4_batch *batch, i
                                  : stream_columns<T, 128, 128>(a, batch, nt, st);
 }
 
+// Workspace of the streaming kernel.
+int64_t stream_bytes(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
+    const int nt = columns_of(c, b, q_heads);
+    const int64_t warps = (nt == 1 ? share_of<1>() : share_of<2>()) * kWarps;
+    return (int64_t)header_bytes(b) + warps * 2 * (16 * nt + nt * c->head_dim * 8) * 4;
+}
+
+// Items of the prompt kernel at most: the sum over sequences of ceil(rows / kPromptRows).
+int64_t prompt_items(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads, int64_t tokens) {
+    const int64_t ratio = q_heads / c->kv_heads, most = cdiv(b->max_tokens * ratio, kPromptRows) * b->sequences;
+    const int64_t bound = cdiv(tokens * ratio, kPromptRows) + b->sequences - 1;
+    return (bound < most ? bound : most) * c->kv_heads;
+}
+
 int check_heads(const oq_kv4_cache *c, int q_heads) {
     OQ_REQUIRE(q_heads >= 1 && q_heads % c->kv_heads == 0, "kv4_attention: q_heads must be a multiple of kv_heads");
     return OQ_OK;
@@ -719,12 +733,17 @@ int check_heads(const oq_kv4_cache *c, int q_heads) {
 using namespace oq;
 using namespace oq::kv4;
 
-extern "C" int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
-                                                    int q_heads) {
-    if (check_cache(cache) || check_batch(batch, 1) || check_heads(cache, q_heads)) return 0;
-    const int nt = columns_of(cache, batch, q_heads);
-    const int64_t share = nt == 1 ? share_of<1>() : share_of<2>();
-    return (int64_t)header_bytes(batch) + share * kWarps * 2 * (16 * nt + nt * cache->head_dim * 8) * 4;
+extern "C" int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache, const oq_kv4_batch *batch, int q_heads,
+                                                    int64_t tokens) {
+    clear_error();
+    if (check_cache(cache) || check_batch(batch, tokens) || check_heads(cache, q_heads)) return 0;
+    const int64_t ratio = q_heads / cache->kv_heads;
+    int64_t n = stream_bytes(cache, batch, q_heads);
+    if (batch->max_tokens * ratio > (ratio > kFew ? ratio : kFew)) {
+        const int64_t items = prompt_items(cache, batch, q_heads, tokens);
+        n += prompt_part_bytes(cache, items, prompt_cuts(cache, batch, items));
+    }
+    return n;
 }
 
 extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *batch, const void *q, int dtype,
@@ -741,7 +760,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     OQ_REQUIRE(window >= 0, "kv4_attention: window must not be negative");
     OQ_REQUIRE((flags & ~OQ_KV4_NOT_CAUSAL) == 0, "kv4_attention: unknown flags");
     OQ_REQUIRE(scale == scale && scale - scale == 0.0f, "kv4_attention: scale must be finite");
-    OQ_REQUIRE((int64_t)ws_bytes >= oq_kv4_attention_workspace_bytes(cache, batch, q_heads),
+    OQ_REQUIRE((int64_t)ws_bytes >= oq_kv4_attention_workspace_bytes(cache, batch, q_heads, tokens),
                "kv4_attention: workspace too small");
     Args a = {};
     a.k_codes = cache->k_codes;
@@ -771,9 +790,10 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;  // rows a sequence and key head
     a.few = a.ratio > kFew ? a.ratio : kFew;                   // single tokens are always streamed
     if (most > a.few) {
-        // sum over sequences of ceil(rows / kPromptRows), at most
-        const int64_t items = (cdiv(tokens * a.ratio, kPromptRows) + batch->sequences) * a.kv_heads;
-        if (int rc = prompt_attention(a, dtype, cache, batch->sequences, items, st)) return rc;
+        AttnArgs p = a;
+        p.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + stream_bytes(cache, batch, q_heads));
+        const int64_t items = prompt_items(cache, batch, q_heads, tokens);
+        if (int rc = prompt_attention(p, dtype, cache, items, prompt_cuts(cache, batch, items), st)) return rc;
     }
     return dtype == OQ_F16 ? attention_typed<__half>(a, cache, batch, nt, st)
                            : attention_typed<__nv_bfloat16>(a, cache, batch, nt, st);

@@ -74,10 +74,13 @@ __device__ __forceinline__ float fp16_power(float top, float &down) {
 }
 
 // The prompt kernel over every sequence with more than a.few query rows.
-// `items`: an upper bound of its (sequence, key head, row block) items.
-int prompt_attention(const AttnArgs &a, int dtype, const oq_kv4_cache *c, int sequences, int64_t items,
-                     cudaStream_t st);
+// `items`: an upper bound of its (sequence, key head, row block) items, each
+// of which is cut into up to `cuts` parts of its cached tokens.
 constexpr int kPromptRows = 256;  // query rows of an item
+constexpr int kMostCuts = 64;
+int prompt_cuts(const oq_kv4_cache *c, const oq_kv4_batch *b, int64_t items);
+int64_t prompt_part_bytes(const oq_kv4_cache *c, int64_t items, int cuts);
+int prompt_attention(const AttnArgs &a, int dtype, const oq_kv4_cache *c, int64_t items, int cuts, cudaStream_t st);
 
 }  // namespace kv4
 }  // namespace oq

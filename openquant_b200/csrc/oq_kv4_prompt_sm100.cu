@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 512;
 constexpr int kTok = 128;   // cached tokens of a block
+constexpr int kLeastBlocks = 3;  // of a part
 constexpr int kStages = 2;  // K and V tiles in shared memory
 constexpr uint32_t kTmemCols = 512;
 // TMEM columns: S buffers (tile, block & 1) of kTok at 0, O tiles at 256 and 256 + head_dim
@@ -81,6 +82,32 @@ __device__ __forceinline__ bool elect_one() {
     return v != 0;
 }
 
+// 16 bytes that are read once: no line of the (small) L1 is taken for them.
+__device__ __forceinline__ uint4 ld16_once(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
+// mbar_wait() that looks at the clock and at the error word (a global load
+// that all waiting warps of the GPU would share) only every 256th time; the
+// hardware suspends a try for a while, so that stays far below the limit's
+// resolution.
+__device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
+    const uint32_t a = smem_u32(bar);
+    if (mbar_try_wait(a, parity)) return true;
+    const long long t0 = clock64();
+    for (int i = 1;; ++i) {
+        if (mbar_try_wait(a, parity)) return true;
+        if ((i & 255) == 0 && (clock64() - t0 > kWaitCycles || *(volatile int *)&g_device_error != 0)) {
+            record_device_error(OQ_DEV_TIMEOUT);
+            return false;
+        }
+    }
+}
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // Byte offset of the 16-byte chunk `c` (eight elements) of row r.
@@ -93,8 +120,77 @@ __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
+// What item `id` (over all sequences with more than a.few rows) works on.
+struct Item {
+    int b, first, count, length, rows, head, row0;
+    int nblk;       // blocks of kTok cached tokens from `lo` on, for all its parts
+    int parts;      // parts it is cut into
+    int floor, lo, hi;  // first visible token, the same down to 16, one past the last
+};
+
+// Finds it with all THREADS threads of the CTA; false: there is no such item.
+template <int THREADS>
+__device__ __forceinline__ bool find_item(const AttnArgs &a, int id, int cuts, Item &it) {
+    __shared__ int warp_sum[THREADS / 32], found[2];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int base = 0;
+    if (tid == 0) found[0] = -1;
+    __syncthreads();
+    for (int b0 = 0; b0 < a.batch.sequences; b0 += THREADS) {
+        const int b = b0 + tid;
+        int n = 0;
+        if (b < a.batch.sequences) {
+            int first, count;
+            tokens_of(a.batch, b, a.tokens, first, count);
+            const int64_t rows = (int64_t)count * a.ratio;
+            if (rows > a.few) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
+        }
+        int inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_sum[warp] = inc;
+        __syncthreads();
+        int before = base;
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += warp_sum[w];
+            base += warp_sum[w];
+        }
+        before += inc - n;
+        if (id >= before && id < before + n) {
+            found[0] = b;
+            found[1] = id - before;
+        }
+        __syncthreads();
+    }
+    it.b = found[0];
+    if (it.b < 0) return false;
+    tokens_of(a.batch, it.b, a.tokens, it.first, it.count);
+    it.length = length_of(a.batch, it.b, a.page_size);
+    it.rows = it.count * a.ratio;
+    const int blocks = (it.rows + kPromptRows - 1) / kPromptRows;
+    // the last rows see most: they go first
+    it.head = found[1] % a.kv_heads;
+    it.row0 = (blocks - 1 - found[1] / a.kv_heads) * kPromptRows;
+    const int last = min(it.row0 + kPromptRows, it.rows) - 1, base_pos = it.length - it.count;
+    const int p0 = base_pos + it.row0 / a.ratio, p1 = base_pos + last / a.ratio;
+    it.hi = a.causal ? p1 + 1 : it.length;
+    it.floor = a.window > 0 ? (int)max((int64_t)p0 + 1 - a.window, (int64_t)0) : 0;
+    it.lo = it.floor & ~15;
+    it.nblk = it.hi > it.lo ? (it.hi - it.lo + kTok - 1) / kTok : 0;
+    it.parts = max(min(cuts, it.nblk / kLeastBlocks), 1);
+    return true;
+}
+
+// A part of an item: m[256], l[256], then O as float4 [HD / 4][256 rows]
+// (columns in the order of TMEM).
+template <int HD>
+constexpr int kPartFloats = kPromptRows * (HD + 2);
+
 template <typename T, int HD, int GS>
-__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_constant__ AttnArgs a, int cuts) {
     using L = Smem<HD>;
     constexpr int NG = HD / GS, CH = HD / 32;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -108,57 +204,16 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     static_assert((12 + 4 * kStages) * 8 + 4 <= 256, "barrier space");
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
-    // ---- this CTA's item: items before each sequence, then the sequence
-    __shared__ int warp_sum[kThreads / 32], found[2];
-    {
-        int base = 0;
-        if (tid == 0) found[0] = -1;
-        __syncthreads();
-        for (int b0 = 0; b0 < a.batch.sequences; b0 += kThreads) {
-            const int b = b0 + tid;
-            int n = 0;
-            if (b < a.batch.sequences) {
-                int first, count;
-                tokens_of(a.batch, b, a.tokens, first, count);
-                const int64_t rows = (int64_t)count * a.ratio;
-                if (rows > a.few) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
-            }
-            int inc = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
-            }
-            if (lane == 31) warp_sum[warp] = inc;
-            __syncthreads();
-            int before = base;
-            for (int w = 0; w < kThreads / 32; ++w) {
-                if (w < warp) before += warp_sum[w];
-                base += warp_sum[w];
-            }
-            before += inc - n;
-            if ((int)blockIdx.x >= before && (int)blockIdx.x < before + n) {
-                found[0] = b;
-                found[1] = blockIdx.x - before;
-            }
-            __syncthreads();
-        }
-    }
-    const int b = found[0];
-    if (b < 0) return;
-    int first, count;
-    tokens_of(a.batch, b, a.tokens, first, count);
-    const int length = length_of(a.batch, b, a.page_size);
-    const int rows = count * a.ratio, blocks = (rows + kPromptRows - 1) / kPromptRows;
-    // the last rows see most: they go first
-    const int head = found[1] % a.kv_heads, row0 = (blocks - 1 - found[1] / a.kv_heads) * kPromptRows;
+    Item it;
+    const int part = blockIdx.x % cuts;
+    if (!find_item<kThreads>(a, blockIdx.x / cuts, cuts, it) || part >= it.parts) return;
+    const int b = it.b, first = it.first, length = it.length, rows = it.rows, head = it.head, row0 = it.row0;
     const int nrows = min(kPromptRows, rows - row0);
-    const int64_t base = (int64_t)length - count;  // position of the step's first token
-    const int64_t p0 = base + row0 / a.ratio, p1 = base + (row0 + nrows - 1) / a.ratio;
-    const int64_t hi = a.causal ? p1 + 1 : length;
-    const int64_t floor = a.window > 0 ? max(p0 + 1 - a.window, (int64_t)0) : 0;
-    const int64_t lo = floor & ~15ll;
-    const int nblk = hi > lo ? (int)((hi - lo + kTok - 1) / kTok) : 0;
+    const int64_t base = (int64_t)length - it.count;  // position of the step's first token
+    // this part's blocks
+    const int j0 = (int)((int64_t)part * it.nblk / it.parts), j1 = (int)((int64_t)(part + 1) * it.nblk / it.parts);
+    const int nblk = j1 - j0;
+    const int64_t floor = it.floor, lo = it.lo + (int64_t)j0 * kTok, hi = min(it.hi, it.lo + j1 * kTok);
     const int tiles = nrows > 128 ? 2 : 1;
 
     if (tid == 0) {
@@ -195,31 +250,60 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const bool in = row < rows;
         if (wg < tiles) {
             const int tk = in ? row / a.ratio : 0;
+            constexpr int LPR = HD / 8, PER = 32 / LPR;  // lanes a row, rows a step of the warp
+            const int sub = lane / LPR, c = lane % LPR;
+            // this thread's row in q (elements), and in the output and the log-sums (rows)
+            const int64_t q_at = (int64_t)(first + tk) * a.q_ts +
+                                 (int64_t)(head * a.ratio + (in ? row - tk * a.ratio : 0)) * a.q_hs;
             const int64_t at = (int64_t)(first + tk) * a.q_heads + head * a.ratio + (in ? row - tk * a.ratio : 0);
+            const int live = min(max(rows - (row0 + wg * 128 + (warp & 3) * 32), 0), 32);  // rows of the warp
             float f = fabsf(a.f);
             {
-                const T *src = static_cast<const T *>(a.q) + (int64_t)(first + tk) * a.q_ts +
-                               (int64_t)(head * a.ratio + (in ? row - tk * a.ratio : 0)) * a.q_hs;
-                float top = 0.0f, v[8], down;
-                if (!std::is_same<T, __half>::value && in) {
-                    for (int c = 0; c < HD / 8; ++c) {
-                        load_q8<T>(src + 8 * c, a.vec, v);
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
-                    }
-                }
-                float up = fp16_power<T>(top, down);
-                f *= down;
-                if (a.f < 0.0f) up = -up;
+                // The warp's 32 rows, PER at a time, a lane eight elements of one: whole
+                // rows a load, all in flight.
                 const uint32_t dst = smem_u32(smem + L::kQ + wg * L::kQTile);
-                for (int c = 0; c < HD / 8; ++c) {
-                    uint32_t w[4] = {0, 0, 0, 0};
-                    if (in) {
-                        load_q8<T>(src + 8 * c, a.vec, v);
+                constexpr int U = 32 / PER;
+                {
+                    uint4 raw[U];
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        const int n = i * PER + sub;
+                        const int64_t from = __shfl_sync(0xffffffffu, (long long)q_at, n);
+                        if (n < live) {
+                            const T *src = static_cast<const T *>(a.q) + from + 8 * c;
+                            if (a.vec) {
+                                raw[i] = ld16_once(src);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&raw[i])[e] = src[e];
+                            }
+                        } else {
+                            raw[i] = make_uint4(0, 0, 0, 0);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < U; ++i) {
+                        const int x = i * PER;  // the warp's rows x .. x + PER
+                        float top = 0.0f, down, v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = Elem<T>::to_f32(reinterpret_cast<const T *>(&raw[i])[e]);
+                        if (!std::is_same<T, __half>::value) {
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+#pragma unroll
+                            for (int d = 1; d < LPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                        }
+                        float up = fp16_power<T>(top, down);
+                        if (a.f < 0.0f) up = -up;
+                        if (!std::is_same<T, __half>::value) {  // to the thread that has the row
+                            down = __shfl_sync(0xffffffffu, down, lane % PER * LPR);
+                            if (lane / PER * PER == x) f *= down;
+                        }
+                        uint32_t w[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) w[e] = as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up));
+                        st16(dst + chunk_at<L::kQPanel>((warp & 3) * 32 + x + sub, c), w[0], w[1], w[2], w[3]);
                     }
-                    st16(dst + chunk_at<L::kQPanel>(r, c), w[0], w[1], w[2], w[3]);
                 }
                 fence_async_smem();
                 mbar_arrive(q_full);
@@ -237,7 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             bool ok = true;
             for (int j = 0; j < nblk; ++j) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&s_full[wg], j & 1));
+                ok = __all_sync(0xffffffffu, wait(&s_full[wg], j & 1));
                 if (!ok) break;
                 tc_fence_after();
                 uint32_t s[4][32];
@@ -304,12 +388,31 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const float l = (l2[0].x + l2[0].y) + (l2[1].x + l2[1].y);
             // ------------------------------------------------- epilogue
             if (nblk > 0) {
-                ok = __all_sync(0xffffffffu, ok && mbar_wait(done, 0));
+                ok = __all_sync(0xffffffffu, ok && wait(done, 0));
                 tc_fence_after();
             }
-            if (ok) {
+            if (ok && it.parts > 1) {
+                float *dst = a.parts + (int64_t)blockIdx.x * kPartFloats<HD> + wg * 128 + r;
+                dst[0] = m;
+                dst[kPromptRows] = l;
+                float4 *po = reinterpret_cast<float4 *>(a.parts + (int64_t)blockIdx.x * kPartFloats<HD> + 2 * kPromptRows) +
+                             wg * 128 + r;
+#pragma unroll
+                for (int i = 0; i < HD / 32; ++i) {
+                    uint32_t o[32];
+                    tmem_ld_32x32b_x32(to + 32 * i, o);
+                    tc_wait_ld();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        po[(8 * i + x) * kPromptRows] =
+                            make_float4(__uint_as_float(o[4 * x]), __uint_as_float(o[4 * x + 1]),
+                                        __uint_as_float(o[4 * x + 2]), __uint_as_float(o[4 * x + 3]));
+                }
+            } else if (ok) {
+                // O / l through shared memory (Q's tile: every product is done), so that
+                // whole rows go out
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-                T *dst = static_cast<T *>(a.out) + at * HD;
+                const uint32_t mine = smem_u32(smem + L::kQ + wg * L::kQTile);
 #pragma unroll
                 for (int i = 0; i < HD / 32; ++i) {
                     uint32_t o[32];
@@ -320,16 +423,28 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 #pragma unroll
                         for (int e = 0; e < 32; ++e) o[e] = 0;
                     }
-                    if (in) {
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            alignas(16) T v[8];
+                    for (int x = 0; x < 4; ++x) {
+                        alignas(16) T v[8];
 #pragma unroll
-                            for (int e = 0; e < 8; ++e)  // column e holds element 0 4 1 5 2 6 3 7
-                                put(&v[(e >> 1) + (e & 1) * 4], __uint_as_float(o[8 * c + e]) * inv);
-                            reinterpret_cast<uint4 *>(dst + 32 * i)[c] = *reinterpret_cast<uint4 *>(v);
-                        }
+                        for (int e = 0; e < 8; ++e)  // column e holds element 0 4 1 5 2 6 3 7
+                            put(&v[(e >> 1) + (e & 1) * 4], __uint_as_float(o[8 * x + e]) * inv);
+                        const uint4 w = *reinterpret_cast<uint4 *>(v);
+                        st16(mine + chunk_at<L::kQPanel>(r, 4 * i + x), w.x, w.y, w.z, w.w);
                     }
+                }
+                __syncwarp();
+#pragma unroll 4
+                for (int x = 0; x < 32; x += PER) {
+                    const int rr = (warp & 3) * 32 + x + sub;
+                    const int64_t to_row = __shfl_sync(0xffffffffu, (long long)at, x + sub);
+                    uint4 w;
+                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w)
+                                 : "r"(mine + chunk_at<L::kQPanel>(rr, c))
+                                 : "memory");
+                    if (x + sub < live)
+                        *reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + to_row * HD + 8 * c) = w;
                 }
                 if (in && a.log_sum != nullptr)
                     a.log_sum[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
@@ -371,8 +486,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const uint32_t r16 = __shfl_sync(0xffffffffu, row16, (j % kAhead) * B16 + (tk >> 4));
                 const size_t row = (size_t)r16 * 16 + (tk & 15);
                 const int64_t t = lo + (int64_t)j * kTok + tk;
-                const uint4 w = __ldg(reinterpret_cast<const uint4 *>((keys ? a.k_codes : a.v_codes) + row * (HD / 2) +
-                                                                      c * 16));
+                const uint4 w = ld16_once((keys ? a.k_codes : a.v_codes) + row * (HD / 2) + c * 16);
                 // tokens that no row of the block sees may be anything: they become 0
                 const uint32_t x = t < hi && t >= floor ? (uint32_t)__half_as_ushort(__ldg(
                                                               (keys ? a.k_scales : a.v_scales) + row * NG + c * 32 / GS))
@@ -419,13 +533,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         bool ok = true;
         for (int j = 0; ok && j < nblk; ++j) {
             const int st = j % kStages, turn = j / kStages;
-            if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (turn - 1) & 1));
+            if (turn > 0) ok = __all_sync(0xffffffffu, wait(&k_empty[st], (turn - 1) & 1));
             if (!ok) break;
             store(smem_u32(smem + L::kK + st * L::kTile), kc, true);
             fence_async_smem();
             mbar_arrive(&k_full[st]);
             load(j + 1, true);
-            if (turn > 0) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], (turn - 1) & 1));
+            if (turn > 0) ok = __all_sync(0xffffffffu, wait(&v_empty[st], (turn - 1) & 1));
             if (!ok) break;
             store(smem_u32(smem + L::kV + st * L::kTile), vc, false);
             fence_async_smem();
@@ -469,22 +583,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
                 __syncwarp();
             };
-            bool ok = mbar_wait(q_full, 0) && mbar_wait(&k_full[0], 0);
+            bool ok = wait(q_full, 0) && wait(&k_full[0], 0);
             if (ok) {
                 tc_fence_after();
                 for (int i = 0; i < tiles_u; ++i) scores(i, 0);
             }
             for (int j = 0; ok && j < blocks_u; ++j) {
-                if (!(ok = mbar_wait(&v_full[j % kStages], (j / kStages) & 1))) break;
+                if (!(ok = wait(&v_full[j % kStages], (j / kStages) & 1))) break;
                 for (int i = 0; i < tiles_u; ++i) {
-                    if (!(ok = mbar_wait(&p_full[2 * i], j & 1))) break;
+                    if (!(ok = wait(&p_full[2 * i], j & 1))) break;
                     tc_fence_after();
                     values(i, j, 0);
-                    if (!(ok = mbar_wait(&p_full[2 * i + 1], j & 1))) break;
+                    if (!(ok = wait(&p_full[2 * i + 1], j & 1))) break;
                     tc_fence_after();
                     values(i, j, 1);
                     if (j + 1 < blocks_u) {
-                        if (i == 0 && !(ok = mbar_wait(&k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1))) break;
+                        if (i == 0 && !(ok = wait(&k_full[(j + 1) % kStages], ((j + 1) / kStages) & 1))) break;
                         tc_fence_after();
                         scores(i, j + 1);
                     }
@@ -493,7 +607,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             // Every product this thread issued has completed once `done` fires.
             if (elect_one()) tc_commit(done);
             __syncwarp();
-            mbar_wait(done, 0);
+            wait(done, 0);
         }
         __syncwarp();
         tc_fence_before();
@@ -503,30 +617,94 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     }
 }
 
+// Adds the parts of the items that were cut: a thread a row, 16 columns a CTA.
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPromptRows) join_prompt_kernel(const __grid_constant__ AttnArgs a, int cuts) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    Item it;
+    if (!find_item<kPromptRows>(a, blockIdx.x, cuts, it) || it.parts == 1) return;
+    const int r = threadIdx.x, row = it.row0 + r;
+    if (row >= it.rows) return;
+    const float *src = a.parts + (int64_t)blockIdx.x * cuts * kPartFloats<HD> + r;
+    float m = -1e30f, l = 0.0f;
+    for (int p = 0; p < it.parts; ++p) m = fmaxf(m, src[(int64_t)p * kPartFloats<HD>]);
+    float4 o[4] = {};
+#pragma unroll 2
+    for (int p = 0; p < it.parts; ++p) {
+        const float *part = src + (int64_t)p * kPartFloats<HD>;
+        const float c = ex2(part[0] - m);
+        l = fmaf(c, part[kPromptRows], l);
+        const float4 *po = reinterpret_cast<const float4 *>(part - r + 2 * kPromptRows) + blockIdx.y * 4 * kPromptRows + r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float4 v = po[i * kPromptRows];
+            o[i].x = fmaf(c, v.x, o[i].x), o[i].y = fmaf(c, v.y, o[i].y);
+            o[i].z = fmaf(c, v.z, o[i].z), o[i].w = fmaf(c, v.w, o[i].w);
+        }
+    }
+    const int tk = row / a.ratio;
+    const int64_t at = (int64_t)(it.first + tk) * a.q_heads + it.head * a.ratio + (row - tk * a.ratio);
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    T *dst = static_cast<T *>(a.out) + at * HD + blockIdx.y * 16;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // eight columns hold elements 0 4 1 5 2 6 3 7
+        alignas(16) T v[8];
+        const float4 x = o[2 * h], y = o[2 * h + 1];
+        put(&v[0], x.x * inv), put(&v[4], x.y * inv), put(&v[1], x.z * inv), put(&v[5], x.w * inv);
+        put(&v[2], y.x * inv), put(&v[6], y.y * inv), put(&v[3], y.z * inv), put(&v[7], y.w * inv);
+        reinterpret_cast<uint4 *>(dst)[h] = *reinterpret_cast<uint4 *>(v);
+    }
+    if (blockIdx.y == 0 && a.log_sum != nullptr)
+        a.log_sum[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+
 template <typename T, int HD, int GS>
-int launch(const AttnArgs &a, int64_t items, cudaStream_t st) {
+int launch(const AttnArgs &a, int64_t items, int cuts, cudaStream_t st) {
     auto kern = prompt_kernel<T, HD, GS>;
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void *>(kern), Smem<HD>::kBytes)) return rc;
-    kern<<<(unsigned)items, kThreads, Smem<HD>::kBytes, st>>>(a);
-    return check_launch("kv4_attention (prompt)");
+    kern<<<(unsigned)(items * cuts), kThreads, Smem<HD>::kBytes, st>>>(a, cuts);
+    if (int rc = check_launch("kv4_attention (prompt)")) return rc;
+    if (cuts == 1) return OQ_OK;
+    join_prompt_kernel<T, HD><<<dim3((unsigned)items, HD / 16), kPromptRows, 0, st>>>(a, cuts);
+    return check_launch("kv4_attention (prompt join)");
 }
 
 template <typename T>
-int launch_typed(const AttnArgs &a, const oq_kv4_cache *c, int64_t items, cudaStream_t st) {
+int launch_typed(const AttnArgs &a, const oq_kv4_cache *c, int64_t items, int cuts, cudaStream_t st) {
     if (c->head_dim == 64)
-        return c->group_size == 32 ? launch<T, 64, 32>(a, items, st) : launch<T, 64, 64>(a, items, st);
-    return c->group_size == 32   ? launch<T, 128, 32>(a, items, st)
-           : c->group_size == 64 ? launch<T, 128, 64>(a, items, st)
-                                 : launch<T, 128, 128>(a, items, st);
+        return c->group_size == 32 ? launch<T, 64, 32>(a, items, cuts, st) : launch<T, 64, 64>(a, items, cuts, st);
+    return c->group_size == 32   ? launch<T, 128, 32>(a, items, cuts, st)
+           : c->group_size == 64 ? launch<T, 128, 64>(a, items, cuts, st)
+                                 : launch<T, 128, 128>(a, items, cuts, st);
 }
 
 }  // namespace
 
-int prompt_attention(const AttnArgs &a, int dtype, const oq_kv4_cache *c, int sequences, int64_t items,
-                     cudaStream_t st) {
-    (void)sequences;
+// Into how many parts items are cut: what takes the GPU the fewest rounds of
+// a part's blocks and its beginning and end (about kEnds blocks' time), for
+// the longest context that the page table allows.
+int prompt_cuts(const oq_kv4_cache *c, const oq_kv4_batch *b, int64_t items) {
+    constexpr double kEnds = 5.0;
+    const int64_t sms = sm_count(), blocks = cdiv((int64_t)b->max_pages * c->page_size, kTok);
+    if (items >= 4 * sms) return 1;
+    int best = 1;
+    double least = 1e300;
+    for (int n = 1; n <= kMostCuts && n <= blocks / kLeastBlocks + 1; ++n) {
+        // a join costs about as much as a part's ends, too
+        const double t = (double)cdiv(items * n, sms) * ((double)blocks / n + kEnds) + (n > 1 ? kEnds : 0.0);
+        if (t < least) least = t, best = n;
+    }
+    return best;
+}
+
+int64_t prompt_part_bytes(const oq_kv4_cache *c, int64_t items, int cuts) {
+    return cuts == 1 ? 0 : items * cuts * kPromptRows * (c->head_dim + 2) * 4;
+}
+
+int prompt_attention(const AttnArgs &a, int dtype, const oq_kv4_cache *c, int64_t items, int cuts, cudaStream_t st) {
     OQ_REQUIRE(items < (1ll << 31), "kv4_attention: too many query rows");
-    return dtype == OQ_F16 ? launch_typed<__half>(a, c, items, st) : launch_typed<__nv_bfloat16>(a, c, items, st);
+    return dtype == OQ_F16 ? launch_typed<__half>(a, c, items, cuts, st)
+                           : launch_typed<__nv_bfloat16>(a, c, items, cuts, st);
 }
 
 }  // namespace kv4

@@ -260,7 +260,7 @@ class KVBatch:
         self._c = _Batch(page_table.data_ptr(), lengths.data_ptr(), starts.data_ptr() if starts is not None else None,
                          n, int(page_table.shape[1]), max_tokens)
         self._ref = ctypes.byref(self._c)
-        self._ws = {}  # (cache shape, q_heads) -> workspace bytes
+        self._ws = {}  # (cache shape, q_heads, tokens) -> workspace bytes
 
 
 class Int4KVCache:
@@ -312,7 +312,7 @@ class Int4KVCache:
         self._c = _Cache(k_codes.data_ptr(), k_scales.data_ptr(), v_codes.data_ptr(), v_scales.data_ptr(), pages,
                          page_size, kv_heads, head_dim, self.group_size)
         self._ref = ctypes.byref(self._c)
-        self._key = (kv_heads, head_dim)
+        self._key = (kv_heads, head_dim, page_size)
 
     @classmethod
     def allocate(cls, pages, page_size, kv_heads, head_dim, group_size=32, *, device="cuda"):
@@ -436,11 +436,11 @@ class Int4KVCache:
               or not out.is_contiguous()):
             raise ValueError("out must be a contiguous tensor like q")
         log_sum = torch.empty((tokens, heads), dtype=torch.float32, device=self._device) if return_log_sum else None
-        key = (*self._key, heads)
+        key = (*self._key, heads, tokens)
         ws_bytes = batch._ws.get(key)
         if ws_bytes is None:
             with torch.cuda.device(dev):
-                ws_bytes = self._lib.oq_kv4_attention_workspace_bytes(self._ref, batch._ref, heads)
+                ws_bytes = self._lib.oq_kv4_attention_workspace_bytes(self._ref, batch._ref, heads, tokens)
             if ws_bytes <= 0:
                 raise RuntimeError(nat.last_error() or "kv4_attention: no workspace size")
             batch._ws[key] = ws_bytes

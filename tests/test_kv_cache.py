@@ -137,7 +137,7 @@ def test_library_refuses_bad_caches_and_batches(lib, change, message):
                                  nat.OQ_F16, 2, None, None, 0, None),
                lib.oq_kv4_read(ctypes.byref(c), ctypes.byref(b), p, p, nat.OQ_F16, 2, None)):
         assert st == nat.OQ_ERR_INVALID and message in nat.last_error()
-    assert lib.oq_kv4_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), 4) == 0
+    assert lib.oq_kv4_attention_workspace_bytes(ctypes.byref(c), ctypes.byref(b), 4, 2) == 0
 
 
 @pytest.mark.parametrize("change, message", [

@@ -433,6 +433,16 @@ def test_attention_long_context():
     case.check(q, out, lse)
 
 
+@pytest.mark.parametrize("lengths, counts, window", [([5003], [40], 0), ([4100, 700, 130], [33, 64, 129], 0),
+                                                     ([3000, 2999], [300, 1], 1500)])
+def test_attention_few_rows_over_long_contexts(lengths, counts, window):
+    """Too few rows for the GPU: their cached tokens are shared out and joined."""
+    case = Case(lengths, counts, 1, 64, page=32, junk=True)
+    q = case.queries(2, 64, torch.float16)
+    out, lse = case.cache.attention(q, case.batch, window=window, return_log_sum=True)
+    case.check(q, out, lse, window=window)
+
+
 @pytest.mark.parametrize("count", [1, 200])
 def test_attention_scores_far_apart(count):
     """Scores that grow along the sequence (the running maximum is raised again
