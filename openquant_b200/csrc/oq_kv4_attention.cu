@@ -181,7 +181,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
     const int64_t all = prefix[a.batch.sequences];
     const int64_t shares = shares_of(all, gridDim.x * kWarps);
     const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;  // neighbouring shares on different SMs
-    if (me >= shares) return;
+    if (me >= shares) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // see the end
+        return;
+    }
     const int64_t u0 = me * all / shares, u1 = (me + 1) * all / shares;
 
     for (int64_t u = u0; u < u1;) {
@@ -554,6 +557,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             }
         }
     }
+    // Beside a prompt kernel, this one begins while that still runs (they
+    // depend on nothing of each other), and must not be complete before it.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
 // Adds the parts of the items that more than one warp worked on, in order.  A
@@ -661,29 +667,37 @@ int columns_of(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
 }
 
 template <typename T, int HD, int GS, int NT>
-int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
+int stream_launch(Args &a, const oq_kv4_batch *batch, bool beside, cudaStream_t st) {
     const int share = share_of<NT>();
     auto kern = stream_kernel<T, HD, GS, NT>;
     const size_t smem = ring_bytes<HD, GS>() + (batch->sequences + 1) * 8;  // the prefix follows the rings
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void *>(kern), smem)) return rc;
-    kern<<<share, kWarps * 32, smem, st>>>(a);
-    if (int rc = check_launch("kv4_attention")) return rc;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(share);
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = beside ? 1 : 0;
+    cudaError_t err = cudaLaunchKernelEx(&cfg, kern, (const Args)a);
+    if (err != cudaSuccess) {
+        set_error("kv4_attention: launch failed: %s", cudaGetErrorString(err));
+        return OQ_ERR_CUDA;
+    }
 
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;
     const int64_t blocks = cdiv(most < a.few ? most : a.few, 8 * NT), items = blocks * a.kv_heads;
     OQ_REQUIRE(items <= 65535, "kv4_attention: too many key heads");
     const int warps = share * kWarps;
     const bool split = warps > 16 * items * batch->sequences;
-    cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(split ? Shape<HD, NT>::kSlices : 1, (unsigned)items, batch->sequences);
     cfg.blockDim = dim3(256);
-    cfg.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
+    cfg.dynamicSmemBytes = 0;
     cfg.numAttrs = 1;
-    cudaError_t err = split ? cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, true>, a, warps)
+    err = split ? cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, true>, a, warps)
                             : cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, false>, a, warps);
     if (err != cudaSuccess) {
         set_error("kv4_attention (join): launch failed: %s", cudaGetErrorString(err));
@@ -693,18 +707,20 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, cudaStream_t st) {
 }
 
 template <typename T, int HD, int GS>
-int stream_columns(Args &a, const oq_kv4_batch *batch, int nt, cudaStream_t st) {
-    return nt == 1 ? stream_launch<T, HD, GS, 1>(a, batch, st) : stream_launch<T, HD, GS, 2>(a, batch, st);
+int stream_columns(Args &a, const oq_kv4_batch *batch, int nt, bool beside, cudaStream_t st) {
+    return nt == 1 ? stream_launch<T, HD, GS, 1>(a, batch, beside, st)
+                   : stream_launch<T, HD, GS, 2>(a, batch, beside, st);
 }
 
 template <typename T>
-int attention_typed(Args &a, const oq_kv4_cache *c, const oq_kv4_batch *batch, int nt, cudaStream_t st) {
+int attention_typed(Args &a, const oq_kv4_cache *c, const oq_kv4_batch *batch, int nt, bool beside,
+                    cudaStream_t st) {
     if (c->head_dim == 64)
-        return c->group_size == 32 ? stream_columns<T, 64, 32>(a, batch, nt, st)
-                                   : stream_columns<T, 64, 64>(a, batch, nt, st);
-    return c->group_size == 32   ? stream_columns<T, 128, 32>(a, batch, nt, st)
-           : c->group_size == 64 ? stream_columns<T, 128, 64>(a, batch, nt, st)
-                                 : stream_columns<T, 128, 128>(a, batch, nt, st);
+        return c->group_size == 32 ? stream_columns<T, 64, 32>(a, batch, nt, beside, st)
+                                   : stream_columns<T, 64, 64>(a, batch, nt, beside, st);
+    return c->group_size == 32   ? stream_columns<T, 128, 32>(a, batch, nt, beside, st)
+           : c->group_size == 64 ? stream_columns<T, 128, 64>(a, batch, nt, beside, st)
+                                 : stream_columns<T, 128, 128>(a, batch, nt, beside, st);
 }
 
 // Workspace of the streaming kernel.
@@ -789,12 +805,13 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;  // rows a sequence and key head
     a.few = a.ratio > kFew ? a.ratio : kFew;                   // single tokens are always streamed
-    if (most > a.few) {
+    const bool beside = most > a.few;
+    if (beside) {
         AttnArgs p = a;
         p.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + stream_bytes(cache, batch, q_heads));
         const int64_t items = prompt_items(cache, batch, q_heads, tokens);
         if (int rc = prompt_attention(p, dtype, cache, items, prompt_cuts(cache, batch, items), st)) return rc;
     }
-    return dtype == OQ_F16 ? attention_typed<__half>(a, cache, batch, nt, st)
-                           : attention_typed<__nv_bfloat16>(a, cache, batch, nt, st);
+    return dtype == OQ_F16 ? attention_typed<__half>(a, cache, batch, nt, beside, st)
+                           : attention_typed<__nv_bfloat16>(a, cache, batch, nt, beside, st);
 }

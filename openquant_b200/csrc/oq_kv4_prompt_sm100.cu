@@ -204,6 +204,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     static_assert((12 + 4 * kStages) * 8 + 4 <= 256, "barrier space");
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
+    asm volatile("griddepcontrol.launch_dependents;");  // the streaming kernel fills the SMs that run out of items
     Item it;
     const int part = blockIdx.x % cuts;
     if (!find_item<kThreads>(a, blockIdx.x / cuts, cuts, it) || part >= it.parts) return;
