@@ -23,9 +23,12 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 4;   // warps a CTA; each works by itself
-constexpr int kStages = 4;  // 16-token stages of a warp: a pair in use, a pair in flight
-constexpr int kSetup = 6;   // cost of beginning an item, in blocks of 16 tokens
-constexpr int kLeast = 10;  // smallest share of a warp, in the same unit
+constexpr int kStages = 4;  // 16-token stages of a warp, in use or in flight
+// Cost of beginning an item and the smallest share of a warp, in blocks of 16
+// tokens.  Measured with 2, 6, 12 and 4 .. 40: 64 ragged sequences 91 / 87 / 86
+// us for the first; one sequence of 1000 tokens and 32 key heads 12 us with a
+// least share of 4, 29 us with 40.
+constexpr int kSetup = 12, kLeast = 4;
 
 using Args = AttnArgs;
 
@@ -113,7 +116,8 @@ __device__ __forceinline__ void write_slice(const Args &a, const Work &w, int he
 // other: ragged lengths load the warps alike, and no warp waits for another.
 // A share begins and ends inside an item, whose parts the joining kernel adds
 // in a fixed order.  A warp streams its blocks through its own ring of cp.async
-// stages, two blocks at a time (two independent chains of products); the rows
+// stages, two blocks at a time (two independent chains of products) or, with two
+// column tiles, one; the rows
 // are staged 16 bytes longer than they are, which makes both the ldmatrix of
 // the keys and the 4- or 8-byte reads of the values free of bank conflicts.
 template <typename T, int HD, int GS, int NT>
@@ -125,9 +129,18 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
     constexpr int kCodes = 16 * kPitch;     // staged codes of 16 tokens
     constexpr int kScales = 16 * NG * 2;
     constexpr int kStage = 2 * kCodes + 2 * kScales;
+    constexpr int H = NT == 1 ? 2 : 1;      // blocks a step: one has two chains of products with NT = 2
+    constexpr int kSteps = kStages / H;     // steps in flight or in use
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
     unsigned char *ring = smem + warp * kStages * kStage;
+    const uint32_t ring_u = smem_u32(ring);
+    // this lane's 16 bytes of a block of codes (or of scales: keys', then
+    // values'), and where they are staged
+    const uint8_t *k_lane = a.k_codes + lane * 16, *v_lane = a.v_codes + lane * 16;
+    const unsigned char *sc_lane =
+        reinterpret_cast<const unsigned char *>(lane < 2 * NG ? a.k_scales : a.v_scales) + lane % (2 * NG) * 16;
+    const uint32_t to_codes = lane / CH * kPitch + lane % CH * 16;
     int64_t *prefix = reinterpret_cast<int64_t *>(smem + kWarps * kStages * kStage);
     asm volatile("griddepcontrol.launch_dependents;");
 
@@ -231,31 +244,23 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         auto load = [&](int i) {
             if (i < nblk) {
                 const uint32_t r16 = __shfl_sync(0xffffffffu, rows16, i & 31);
-                const uint32_t dst = smem_u32(ring) + (i % kStages) * kStage;
-                const uint8_t *ks = a.k_codes + (size_t)r16 * (16 * HD / 2);
-                const uint8_t *vs = a.v_codes + (size_t)r16 * (16 * HD / 2);
+                const uint32_t dst = ring_u + (i % kStages) * kStage;
 #pragma unroll
                 for (int j = 0; j < HD / 64; ++j) {
-                    const int ch = lane + 32 * j;
-                    const uint32_t to = dst + (ch / CH) * kPitch + (ch % CH) * 16;
-                    cp16(to, ks + ch * 16);
-                    cp16(to + kCodes, vs + ch * 16);
+                    cp16(dst + to_codes + j * (32 / CH * kPitch), k_lane + (size_t)r16 * (16 * HD / 2) + j * 512);
+                    cp16(dst + to_codes + j * (32 / CH * kPitch) + kCodes,
+                         v_lane + (size_t)r16 * (16 * HD / 2) + j * 512);
                 }
-                if (lane < 4 * NG) {
-                    const unsigned char *sc = reinterpret_cast<const unsigned char *>(lane < 2 * NG ? a.k_scales
-                                                                                                    : a.v_scales);
-                    cp16(dst + 2 * kCodes + lane * 16, sc + (size_t)r16 * kScales + (lane % (2 * NG)) * 16);
-                }
+                if (lane < 4 * NG) cp16(dst + 2 * kCodes + lane * 16, sc_lane + (size_t)r16 * kScales);
             }
         };
         look_up(0);
         __syncwarp();  // the ring's last reads (of the item before) are done
-        load(0);
-        load(1);
-        cp_commit();
-        load(2);
-        load(3);
-        cp_commit();
+#pragma unroll
+        for (int i = 0; i < kStages; ++i) {
+            load(i);
+            if ((i + 1) % H == 0) cp_commit();
+        }
 
         // ---- queries: column n = 8 j + g of this lane as B fragments
         uint32_t qf[NT][CH][4];
@@ -322,17 +327,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             l[j][0] = l[j][1] = 0.0f;
         }
 
-        for (int i = 0; i < nblk; i += 2) {
-            cp_wait<1>();
+        for (int i = 0; i < nblk; i += H) {
+            cp_wait<kSteps - 1>();
             __syncwarp();
             const int tok = first_tok + i * 16;
 
-            // ---- scores of tokens g and g + 8 of both blocks
-            float s[2][NT][4];
+            // ---- scores of tokens g and g + 8 of the blocks
+            float s[H][NT][4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < H; ++h) {
                 const unsigned char *st = ring + ((i + h) % kStages) * kStage;
-                const uint32_t su = smem_u32(st);
+                const uint32_t su = ring_u + ((i + h) % kStages) * kStage;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -402,11 +407,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             }
 
             // ---- weights p = 2^(s f - m)
-            // some column misses some token of the pair, or the pair is half a one
-            const bool edge = tok + 32 > all_vis || tok < all_low || i + 1 == nblk;
+            // some column misses some token of the blocks, or a block is not there
+            const bool edge = tok + 16 * H > all_vis || tok < all_low || i + H > nblk;
             if (edge) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                for (int h = 0; h < H; ++h)
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             }
             bool raise = false;
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -427,7 +432,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float mx = fmaxf(fmaxf(s[0][j][e], s[0][j][e + 2]), fmaxf(s[1][j][e], s[1][j][e + 2]));
+                        float mx = fmaxf(s[0][j][e], s[0][j][e + 2]);
+                        if (H == 2) mx = fmaxf(mx, fmaxf(s[H - 1][j][e], s[H - 1][j][e + 2]));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -443,9 +449,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                         }
                     }
             }
-            uint32_t pf[2][NT][2];
+            uint32_t pf[H][NT][2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < H; ++h)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float p[4];
@@ -460,7 +466,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
 
             // ---- o += V^T p: rows d = HD/8 g + ..., tokens 2 t4, +1, +8, +9
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+            for (int h = 0; h < H; ++h) {
                 const unsigned char *vc = ring + ((i + h) % kStages) * kStage + kCodes;
                 const __half *vsc = reinterpret_cast<const __half *>(vc + kCodes + kScales);
                 constexpr int W = HD / 64;  // words a lane takes of a token
@@ -512,10 +518,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                 }
             }
             __syncwarp();
-            // the next pair but one takes the place of this one
-            if (((i + 4) & 31) == 0) look_up(i + 4);
-            load(i + 4);
-            load(i + 5);
+            // later blocks take the place of these
+            if (((i + kStages) & 31) == 0) look_up(i + kStages);
+#pragma unroll
+            for (int h = 0; h < H; ++h) load(i + kStages + h);
             cp_commit();
         }
         cp_wait<0>();
