@@ -68,6 +68,47 @@ __device__ __forceinline__ int64_t shares_of(int64_t all, int warps) {
     return n < warps ? (n > 0 ? n : 1) : warps;
 }
 
+// Units before each sequence, and all of them: prefix[0 .. sequences] in shared
+// memory, by the CTA's THREADS threads.
+template <int THREADS>
+__device__ __forceinline__ void units_before(const Args &a, int cols, int64_t *prefix) {
+    __shared__ int64_t warp_sum[THREADS / 32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.batch.sequences; b0 += THREADS) {
+        const int b = b0 + tid;
+        int64_t n = 0;
+        if (b < a.batch.sequences) {
+            const Work w = work_of(a, b, cols);
+            n = (int64_t)(w.nb + kSetup) * w.blocks * a.kv_heads;
+        }
+        int64_t inc = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += v;
+        }
+        if (lane == 31) warp_sum[warp] = inc;
+        __syncthreads();
+        int64_t before = base;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; ++w) {
+            if (w < warp) before += warp_sum[w];
+            base += warp_sum[w];
+        }
+        if (b < a.batch.sequences) prefix[b] = before + inc - n;
+        __syncthreads();
+    }
+    if (tid == 0) prefix[a.batch.sequences] = base;
+    __syncthreads();
+}
+
+// x / y for y > 0, in 32 bits where that does (the usual case; 64-bit
+// divisions are a hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
+
 __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
@@ -144,40 +185,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
     int64_t *prefix = reinterpret_cast<int64_t *>(smem + kWarps * kStages * kStage);
     asm volatile("griddepcontrol.launch_dependents;");
 
-    // ---- units before each sequence (exclusive prefix in shared memory)
-    {
-        __shared__ int64_t warp_sum[kWarps];
-        int64_t base = 0;
-        for (int b0 = 0; b0 < a.batch.sequences; b0 += kWarps * 32) {
-            const int b = b0 + tid;
-            int64_t n = 0;
-            if (b < a.batch.sequences) {
-                const Work w = work_of(a, b, kCols);
-                n = (int64_t)(w.nb + kSetup) * w.blocks * a.kv_heads;
-            }
-            int64_t inc = n;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += v;
-            }
-            if (lane == 31) warp_sum[warp] = inc;
-            __syncthreads();
-            int64_t before = base, all = 0;
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                if (w < warp) before += warp_sum[w];
-                all += warp_sum[w];
-            }
-            if (b < a.batch.sequences) prefix[b] = before + inc - n;
-            base += all;
-            __syncthreads();
-        }
-        if (tid == 0) prefix[a.batch.sequences] = base;
-        __syncthreads();
-        if (blockIdx.x == 0)
-            for (int b = tid; b <= a.batch.sequences; b += kWarps * 32) a.prefix[b] = prefix[b];
-    }
+    units_before<kWarps * 32>(a, kCols, prefix);
 
     // Padding tokens: 0, log-sum -inf.
     {
@@ -198,7 +206,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         asm volatile("griddepcontrol.wait;" ::: "memory");  // see the end
         return;
     }
-    const int64_t u0 = me * all / shares, u1 = (me + 1) * all / shares;
+    const int64_t u0 = quotient(me * all, shares), u1 = quotient((me + 1) * all, shares);
 
     for (int64_t u = u0; u < u1;) {
         // ---- the item of unit u
@@ -216,7 +224,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         }
         const Work w = work_of(a, b, kCols);
         const int64_t local = u - prefix[b];
-        const int per = w.nb + kSetup, item = (int)(local / per), off = (int)(local - (int64_t)item * per);
+        const int per = w.nb + kSetup, item = (int)quotient(local, per), off = (int)(local - (int64_t)item * per);
         const int take = (int)min((int64_t)(per - off), u1 - u);
         const int i0 = max(off - kSetup, 0), i1 = off + take - kSetup;  // blocks [i0, i1) of the item
         const int slot = u == u0 ? 0 : 1;  // a part is the share's first item or its last
@@ -576,50 +584,47 @@ template <typename T, int HD, int NT, bool SPLIT>
 __global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
     using S = Shape<HD, NT>;
     constexpr int kCols = S::kCols;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    // All but the parts is known before the streaming kernel is done.
+    extern __shared__ __align__(16) unsigned char join_smem[];
+    int64_t *prefix = reinterpret_cast<int64_t *>(join_smem);
+    units_before<256>(a, kCols, prefix);
     const int b = blockIdx.z, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t4 = lane & 3;
     const Work w = work_of(a, b, kCols);
     const int item = blockIdx.y;
-    if (item >= w.blocks * a.kv_heads) return;
-    const int64_t all = a.prefix[a.batch.sequences], shares = shares_of(all, warps);
-    const int64_t s = a.prefix[b] + (int64_t)item * (w.nb + kSetup), e = s + w.nb + kSetup;
+    const bool there = item < w.blocks * a.kv_heads;
+    const int64_t all = max(prefix[a.batch.sequences], (int64_t)1), shares = shares_of(all, warps);
+    const int64_t s = prefix[b] + (int64_t)item * (w.nb + kSetup), e = s + w.nb + kSetup;
     // the warp that worked on unit u: the last i with i all / shares <= u
-    const int64_t c0 = ((s + kSetup + 1) * shares - 1) / all, c1 = (e * shares - 1) / all;
-    if (c0 == c1) return;
+    const int64_t c0 = quotient((s + kSetup + 1) * shares - 1, all), c1 = quotient(e * shares - 1, all);
     // (every warp between them has units, as shares <= all; only the first may start before the item)
+    const bool late = quotient(c0 * all, shares) >= s;
+    // (also by a CTA that has nothing to do: this kernel is not complete before the other)
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (!there || c0 == c1) return;
     const int head = item / w.blocks, row0 = (item - head * w.blocks) * kCols;
-    const float *first = a.parts + (c0 * 2 + (c0 * all / shares >= s ? 0 : 1)) * S::kPart;
+    const float *first = a.parts + (c0 * 2 + (late ? 0 : 1)) * S::kPart;
     const float *rest = a.parts + c0 * 2 * S::kPart;  // part n > 0: rest + n * 2 * kPart
     const int parts = (int)(c1 - c0) + 1;
     __shared__ float4 so[8][32];
-    __shared__ float sl[8][kCols];
+    __shared__ float sm[8][kCols], sl[8][kCols];
     for (int sl_i = SPLIT ? (int)blockIdx.x : warp; sl_i < S::kSlices; sl_i += SPLIT ? S::kSlices : 8) {
         const int j = sl_i / (HD / 16), i = sl_i % (HD / 16), col = 8 * j + 2 * t4;
         const bool in = row0 + col < w.rows;
-        // the largest m of each of the lane's two columns
+        // of the lane's two columns, over the parts so far
         float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (in) {
-            for (int n = g; n < parts; n += 8) {
-                const float *p = n == 0 ? first : rest + (int64_t)n * 2 * S::kPart;
-                m[0] = fmaxf(m[0], p[col]);
-                m[1] = fmaxf(m[1], p[col + 1]);
-            }
-        }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) m[x] = fmaxf(m[x], __shfl_xor_sync(0xffffffffu, m[x], d));
-        if (in) {
-            constexpr int U = 4;  // parts in flight
+            constexpr int U = 8;  // parts in flight
             for (int n0 = SPLIT ? warp : 0; n0 < parts; n0 += SPLIT ? 8 * U : U) {
                 float4 v[U];
-                float pm[U][2], pl[U][2];
+                float pm[U][2], pl[U][2], mn[2] = {m[0], m[1]};
 #pragma unroll
                 for (int x = 0; x < U; ++x) {
                     const int n = n0 + (SPLIT ? 8 * x : x);
                     const float *p = n == 0 ? first : rest + (int64_t)n * 2 * S::kPart;
+                    v[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     pm[x][0] = pm[x][1] = -INFINITY;
+                    pl[x][0] = pl[x][1] = 0.0f;
                     if (n < parts) {
                         v[x] = reinterpret_cast<const float4 *>(p + 2 * kCols)[sl_i * 32 + lane];
                         pm[x][0] = p[col], pm[x][1] = p[col + 1];
@@ -627,26 +632,44 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
                     }
                 }
 #pragma unroll
+                for (int x = 0; x < U; ++x) mn[0] = fmaxf(mn[0], pm[x][0]), mn[1] = fmaxf(mn[1], pm[x][1]);
+                const float k0 = ex2(m[0] - mn[0]), k1 = ex2(m[1] - mn[1]);
+                m[0] = mn[0], m[1] = mn[1];
+                l[0] *= k0, o.x *= k0, o.z *= k0;
+                l[1] *= k1, o.y *= k1, o.w *= k1;
+#pragma unroll
                 for (int x = 0; x < U; ++x) {
-                    if (n0 + (SPLIT ? 8 * x : x) < parts) {
-                        const float c = ex2(pm[x][0] - m[0]), d = ex2(pm[x][1] - m[1]);
-                        l[0] = fmaf(c, pl[x][0], l[0]);
-                        l[1] = fmaf(d, pl[x][1], l[1]);
-                        o.x = fmaf(c, v[x].x, o.x), o.z = fmaf(c, v[x].z, o.z);
-                        o.y = fmaf(d, v[x].y, o.y), o.w = fmaf(d, v[x].w, o.w);
-                    }
+                    const float c = ex2(pm[x][0] - m[0]), d = ex2(pm[x][1] - m[1]);
+                    l[0] = fmaf(c, pl[x][0], l[0]);
+                    l[1] = fmaf(d, pl[x][1], l[1]);
+                    o.x = fmaf(c, v[x].x, o.x), o.z = fmaf(c, v[x].z, o.z);
+                    o.y = fmaf(d, v[x].y, o.y), o.w = fmaf(d, v[x].w, o.w);
                 }
             }
         }
         if (SPLIT) {
             so[warp][lane] = o;
-            if (g == 0) sl[warp][col] = l[0], sl[warp][col + 1] = l[1];
+            if (g == 0) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) sm[warp][col + x] = m[x], sl[warp][col + x] = l[x];
+            }
             __syncthreads();
             if (warp != 0) return;
-            for (int k = 1; k < 8; ++k) {
-                l[0] += sl[k][col], l[1] += sl[k][col + 1];
-                o.x += so[k][lane].x, o.y += so[k][lane].y, o.z += so[k][lane].z, o.w += so[k][lane].w;
+            float mn[2] = {m[0], m[1]};
+#pragma unroll
+            for (int k = 1; k < 8; ++k) mn[0] = fmaxf(mn[0], sm[k][col]), mn[1] = fmaxf(mn[1], sm[k][col + 1]);
+            l[0] = l[1] = 0.0f;
+            o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float c = ex2(sm[k][col] - mn[0]), d = ex2(sm[k][col + 1] - mn[1]);
+                const float4 v = so[k][lane];
+                l[0] = fmaf(c, sl[k][col], l[0]);
+                l[1] = fmaf(d, sl[k][col + 1], l[1]);
+                o.x = fmaf(c, v.x, o.x), o.z = fmaf(c, v.z, o.z);
+                o.y = fmaf(d, v.y, o.y), o.w = fmaf(d, v.w, o.w);
             }
+            m[0] = mn[0], m[1] = mn[1];
         }
         write_slice<T, HD>(a, w, head, row0 + col, HD / 8 * g + 2 * i, o.x, o.z, m[0], l[0]);
         write_slice<T, HD>(a, w, head, row0 + col + 1, HD / 8 * g + 2 * i, o.y, o.w, m[1], l[1]);
@@ -661,8 +684,6 @@ template <int HD, int GS>
 constexpr size_t ring_bytes() {
     return (size_t)kWarps * kStages * (2 * 16 * (HD / 2 + 16) + 2 * 16 * (HD / GS) * 2);
 }
-
-size_t header_bytes(const oq_kv4_batch *b) { return (size_t)cdiv((b->sequences + 1) * 8, 128) * 128; }
 
 // Sequences of up to kFew query rows a key head are streamed, the others go to
 // the prompt kernel.
@@ -701,7 +722,7 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, bool beside, cudaStream_t 
     const bool split = warps > 16 * items * batch->sequences;
     cfg.gridDim = dim3(split ? Shape<HD, NT>::kSlices : 1, (unsigned)items, batch->sequences);
     cfg.blockDim = dim3(256);
-    cfg.dynamicSmemBytes = 0;
+    cfg.dynamicSmemBytes = (batch->sequences + 1) * 8;
     cfg.numAttrs = 1;
     err = split ? cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, true>, a, warps)
                             : cudaLaunchKernelEx(&cfg, join_kernel<T, HD, NT, false>, a, warps);
@@ -733,7 +754,7 @@ int attention_typed(Args &a, const oq_kv4_cache *c, const oq_kv4_batch *batch, i
 int64_t stream_bytes(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
     const int nt = columns_of(c, b, q_heads);
     const int64_t warps = (nt == 1 ? share_of<1>() : share_of<2>()) * kWarps;
-    return (int64_t)header_bytes(b) + warps * 2 * (16 * nt + nt * c->head_dim * 8) * 4;
+    return warps * 2 * (16 * nt + nt * c->head_dim * 8) * 4;
 }
 
 // Items of the prompt kernel at most: the sum over sequences of ceil(rows / kPromptRows).
@@ -804,8 +825,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     a.f = scale * 1.4426950408889634f;
     a.window = window;
     a.causal = (flags & OQ_KV4_NOT_CAUSAL) ? 0 : 1;
-    a.prefix = static_cast<int64_t *>(workspace);
-    a.parts = reinterpret_cast<float *>(static_cast<char *>(workspace) + header_bytes(batch));
+    a.parts = static_cast<float *>(workspace);
     a.vec = aligned(q, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const int nt = columns_of(cache, batch, q_heads);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

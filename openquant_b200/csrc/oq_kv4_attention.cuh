@@ -24,11 +24,10 @@ struct AttnArgs {
     float f;             // scale * log2 e
     int64_t window;
     int causal;
-    float *parts;     // streaming kernel: partial results, two slots a CTA
-    int64_t *prefix;  // units before each sequence, written by CTA 0 for the joining kernel
-    int vec;          // q rows 16-byte aligned
-    int few;          // sequences of at most `few` query rows a key head go to the streaming kernel,
-                      // the others to the prompt kernel
+    float *parts;  // partial results
+    int vec;       // q rows 16-byte aligned
+    int few;       // sequences of at most `few` query rows a key head go to the streaming kernel,
+                   // the others to the prompt kernel
 };
 
 __device__ __forceinline__ float ex2(float x) {
