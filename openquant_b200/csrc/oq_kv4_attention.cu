@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
         // ---- queries: column n = 8 j + g of this lane as B fragments
         uint32_t qf[NT][CH][4];
         float f[NT][2];            // factor of columns 8 j + 2 t4 and + 1
-        int vis[NT][2], low[NT][2];  // their visible tokens [low, vis)
+        int pos[NT][2];            // their positions
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             const int n = row0 + 8 * j + g;
@@ -310,9 +310,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = row0 + 8 * j + 2 * t4 + e;
-                const int p = w.length - w.count + (col < w.rows ? col / a.ratio : w.count - 1);
-                vis[j][e] = a.causal ? p + 1 : w.length;
-                low[j][e] = a.window > 0 ? (int)max((int64_t)p + 1 - a.window, (int64_t)0) : 0;
+                pos[j][e] = w.length - w.count + (col < w.rows ? col / a.ratio : w.count - 1);
             }
         }
         // tokens that every column of the item sees
@@ -418,14 +416,16 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             // some column misses some token of the blocks, or a block is not there
             const bool edge = tok + 16 * H > all_vis || tok < all_low || i + H > nblk;
             if (edge) {
+                const int64_t window = a.window > 0 ? a.window : INT32_MAX;
 #pragma unroll
                 for (int h = 0; h < H; ++h)
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            const int tk = tok + 16 * h + g + (e >> 1) * 8;
-                            if (tk >= vis[j][e & 1] || tk < low[j][e & 1] || i + h >= nblk) s[h][j][e] = -INFINITY;
+                            const int tk = tok + 16 * h + g + (e >> 1) * 8, p = pos[j][e & 1];
+                            const int vis = a.causal ? p + 1 : w.length;
+                            if (tk >= vis || tk <= p - window || i + h >= nblk) s[h][j][e] = -INFINITY;
                         }
             }
             bool raise = false;

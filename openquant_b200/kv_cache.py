@@ -38,6 +38,7 @@ _CODES = {torch.float32: nat.OQ_F32, torch.float16: nat.OQ_F16, torch.bfloat16: 
 _ROTARY_INTERLEAVED, _ROTARY_INVERSE = 1, 2
 _NOT_CAUSAL = 1
 MAX_SEQUENCES = 2048
+_KEEP_BYTES, _KEEP_STREAMS = 32 << 20, 4  # workspaces that a KVBatch keeps
 
 
 # -------------------------------------------------------------- rotary --
@@ -139,7 +140,7 @@ def _heads(x, name, dtypes=(torch.float16, torch.bfloat16)):
     if not x.is_cuda:
         raise ValueError("All tensors must be on CUDA")
     tokens, heads, dim = x.shape
-    if tokens < 1 or heads < 1 or dim < 1:
+    if not (tokens and heads and dim):
         raise ValueError(f"{name}: dimensions must be positive")
     if x.stride(2) != 1 and dim > 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
@@ -261,6 +262,22 @@ class KVBatch:
                          n, int(page_table.shape[1]), max_tokens)
         self._ref = ctypes.byref(self._c)
         self._ws = {}  # (cache shape, q_heads, tokens) -> workspace bytes
+        self._buffers = {}  # stream -> workspace
+
+
+    def _workspace(self, nbytes, device):
+        """nbytes of scratch memory for a call on the current stream: one buffer
+        per stream, as calls on one stream follow each other; a captured call
+        has its own from the graph's pool, and large ones are not kept."""
+        if nbytes > _KEEP_BYTES or torch.cuda.is_current_stream_capturing():
+            return torch.empty(nbytes, dtype=torch.uint8, device=device)
+        stream = _stream_handle(self._dev)
+        buf = self._buffers.get(stream)
+        if buf is None or buf.numel() < nbytes:
+            if len(self._buffers) >= _KEEP_STREAMS:
+                self._buffers.clear()
+            buf = self._buffers[stream] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        return buf
 
 
 class Int4KVCache:
@@ -444,7 +461,11 @@ class Int4KVCache:
             if ws_bytes <= 0:
                 raise RuntimeError(nat.last_error() or "kv4_attention: no workspace size")
             batch._ws[key] = ws_bytes
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self._device)
+        if torch.cuda.current_device() != dev:  # the workspace is the current stream's
+            with torch.cuda.device(dev):
+                ws = batch._workspace(ws_bytes, self._device)
+        else:
+            ws = batch._workspace(ws_bytes, self._device)
         qs = q.stride()
         _call(dev, self._lib.oq_kv4_attention, self._ref, batch._ref, q.data_ptr(), _CODES[q.dtype], heads, qs[0],
               qs[1], out.data_ptr(), log_sum.data_ptr() if return_log_sum else None, tokens, scale, window,
