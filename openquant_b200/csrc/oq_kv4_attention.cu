@@ -685,9 +685,16 @@ constexpr size_t ring_bytes() {
     return (size_t)kWarps * kStages * (2 * 16 * (HD / 2 + 16) + 2 * 16 * (HD / GS) * 2);
 }
 
-// Sequences of up to kFew query rows a key head are streamed, the others go to
-// the prompt kernel.
-constexpr int kFew = 32;
+// Sequences of up to this many query rows a key head are streamed (in blocks of
+// 16 rows, each of which reads the cache again, from L2), the others go to the
+// prompt kernel, whose tiles have 128 rows.  Single tokens are always streamed.
+// Measured, streamed / prompt kernel: head_dim 64, 37 rows over 23 x 11139
+// tokens 173 / 186 us, 48 rows over 34 x 8902..17804 tokens 52 / 62 us; head_dim
+// 128, 40 rows over 16 x 8000 tokens 154 / 122 us, 64 rows 198 / 123 us.
+int few_rows(const oq_kv4_cache *c, int q_heads) {
+    const int ratio = q_heads / c->kv_heads, few = c->head_dim == 64 ? 64 : 32;
+    return ratio > few ? ratio : few;
+}
 
 int columns_of(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
     return (int64_t)b->max_tokens * (q_heads / c->kv_heads) <= 8 ? 1 : 2;
@@ -782,7 +789,7 @@ extern "C" int64_t oq_kv4_attention_workspace_bytes(const oq_kv4_cache *cache, c
     if (check_cache(cache) || check_batch(batch, tokens) || check_heads(cache, q_heads)) return 0;
     const int64_t ratio = q_heads / cache->kv_heads;
     int64_t n = stream_bytes(cache, batch, q_heads);
-    if (batch->max_tokens * ratio > (ratio > kFew ? ratio : kFew)) {
+    if (batch->max_tokens * ratio > few_rows(cache, q_heads)) {
         const int64_t items = prompt_items(cache, batch, q_heads, tokens);
         n += prompt_part_bytes(cache, items, prompt_cuts(cache, batch, items));
     }
@@ -830,7 +837,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     const int nt = columns_of(cache, batch, q_heads);
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;  // rows a sequence and key head
-    a.few = a.ratio > kFew ? a.ratio : kFew;                   // single tokens are always streamed
+    a.few = few_rows(cache, q_heads);
     const bool beside = most > a.few;
     if (beside) {
         AttnArgs p = a;

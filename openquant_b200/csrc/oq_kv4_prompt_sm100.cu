@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         };
         uint4 kc[N], vc[N];
-        uint32_t sc[N];  // scales of a chunk: K low, V high half
+        unsigned short ks[N], vs[N];  // their scales (nothing is done with what is in flight)
         // chunk i of the thread: token (r + 128 i) / CH, 16-byte chunk (r + 128 i) % CH
         auto load = [&](int j, bool keys) {
             if (j >= nblk) return;
@@ -487,25 +487,24 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 const uint32_t r16 = __shfl_sync(0xffffffffu, row16, (j % kAhead) * B16 + (tk >> 4));
                 const size_t row = (size_t)r16 * 16 + (tk & 15);
                 const int64_t t = lo + (int64_t)j * kTok + tk;
-                const uint4 w = ld16_once((keys ? a.k_codes : a.v_codes) + row * (HD / 2) + c * 16);
                 // tokens that no row of the block sees may be anything: they become 0
-                const uint32_t x = t < hi && t >= floor ? (uint32_t)__half_as_ushort(__ldg(
-                                                              (keys ? a.k_scales : a.v_scales) + row * NG + c * 32 / GS))
-                                                        : 0u;
+                const bool live = t < hi && t >= floor;
                 if (keys) {
-                    kc[i] = w;
-                    sc[i] = (sc[i] & 0xffff0000u) | x;
+                    kc[i] = ld16_once(a.k_codes + row * (HD / 2) + c * 16);
+                    ks[i] = 0;
+                    if (live) ks[i] = __ldg(reinterpret_cast<const unsigned short *>(a.k_scales) + row * NG + c * 32 / GS);
                 } else {
-                    vc[i] = w;
-                    sc[i] = (sc[i] & 0xffffu) | x << 16;
+                    vc[i] = ld16_once(a.v_codes + row * (HD / 2) + c * 16);
+                    vs[i] = 0;
+                    if (live) vs[i] = __ldg(reinterpret_cast<const unsigned short *>(a.v_scales) + row * NG + c * 32 / GS);
                 }
             }
         };
-        auto store = [&](uint32_t dst, const uint4 (&w)[N], bool keys) {
+        auto store = [&](uint32_t dst, const uint4 (&w)[N], const unsigned short (&sc)[N]) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 const int id = r + 128 * i, tk = id / CH, c = id % CH;
-                const __half2 s2 = __half2half2(__ushort_as_half((unsigned short)(keys ? sc[i] & 0xffffu : sc[i] >> 16)));
+                const __half2 s2 = __half2half2(__ushort_as_half(sc[i]));
                 uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
                 // the upper chunks of a row take their words in the order 2 3 0 1:
                 // the eight lanes of a 128-byte store then hit different banks
@@ -527,8 +526,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 }
             }
         };
-#pragma unroll
-        for (int i = 0; i < N; ++i) sc[i] = 0;
         load(0, true);
         load(0, false);
         bool ok = true;
@@ -536,13 +533,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int st = j % kStages, turn = j / kStages;
             if (turn > 0) ok = __all_sync(0xffffffffu, wait(&k_empty[st], (turn - 1) & 1));
             if (!ok) break;
-            store(smem_u32(smem + L::kK + st * L::kTile), kc, true);
+            store(smem_u32(smem + L::kK + st * L::kTile), kc, ks);
             fence_async_smem();
             mbar_arrive(&k_full[st]);
             load(j + 1, true);
             if (turn > 0) ok = __all_sync(0xffffffffu, wait(&v_empty[st], (turn - 1) & 1));
             if (!ok) break;
-            store(smem_u32(smem + L::kV + st * L::kTile), vc, false);
+            store(smem_u32(smem + L::kV + st * L::kTile), vc, vs);
             fence_async_smem();
             mbar_arrive(&v_full[st]);
             load(j + 1, false);
