@@ -477,55 +477,62 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         };
         uint4 kc[N], vc[N];
         unsigned short ks[N], vs[N];  // their scales (nothing is done with what is in flight)
-        // chunk i of the thread: token (r + 128 i) / CH, 16-byte chunk (r + 128 i) % CH
+        // Chunk i of the thread: token r / CH + i * 128 / CH, 16-byte chunk r % CH, so
+        // that all of them have one place within 16 tokens and one swizzle.
+        const int tk0 = r / CH, c = r % CH;
+        const size_t code_at = (size_t)(tk0 & 15) * (HD / 2) + c * 16, scale_at = (size_t)(tk0 & 15) * NG + c * 32 / GS;
+        const uint8_t *k_lane = a.k_codes + code_at, *v_lane = a.v_codes + code_at;
+        const unsigned short *ks_lane = reinterpret_cast<const unsigned short *>(a.k_scales) + scale_at;
+        const unsigned short *vs_lane = reinterpret_cast<const unsigned short *>(a.v_scales) + scale_at;
+        uint32_t r16[N];  // the chunks' rows / 16 in the cache, of block `at_block`
+        auto rows_of = [&](int j) {
+            if (j >= nblk) return;
+            if (j % kAhead == 0) look_up(j);
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                r16[i] = __shfl_sync(0xffffffffu, row16, (j % kAhead) * B16 + ((tk0 + i * (128 / CH)) >> 4));
+        };
         auto load = [&](int j, bool keys) {
             if (j >= nblk) return;
-            if (keys && j % kAhead == 0) look_up(j);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int id = r + 128 * i, tk = id / CH, c = id % CH;
-                const uint32_t r16 = __shfl_sync(0xffffffffu, row16, (j % kAhead) * B16 + (tk >> 4));
-                const size_t row = (size_t)r16 * 16 + (tk & 15);
-                const int64_t t = lo + (int64_t)j * kTok + tk;
                 // tokens that no row of the block sees may be anything: they become 0
+                const int64_t t = lo + (int64_t)j * kTok + tk0 + i * (128 / CH);
                 const bool live = t < hi && t >= floor;
                 if (keys) {
-                    kc[i] = ld16_once(a.k_codes + row * (HD / 2) + c * 16);
+                    kc[i] = ld16_once(k_lane + (size_t)r16[i] * (16 * HD / 2));
                     ks[i] = 0;
-                    if (live) ks[i] = __ldg(reinterpret_cast<const unsigned short *>(a.k_scales) + row * NG + c * 32 / GS);
+                    if (live) ks[i] = __ldg(ks_lane + (size_t)r16[i] * (16 * NG));
                 } else {
-                    vc[i] = ld16_once(a.v_codes + row * (HD / 2) + c * 16);
+                    vc[i] = ld16_once(v_lane + (size_t)r16[i] * (16 * HD / 2));
                     vs[i] = 0;
-                    if (live) vs[i] = __ldg(reinterpret_cast<const unsigned short *>(a.v_scales) + row * NG + c * 32 / GS);
+                    if (live) vs[i] = __ldg(vs_lane + (size_t)r16[i] * (16 * NG));
                 }
             }
         };
+        // the upper chunks of a row take their words in the order 2 3 0 1:
+        // the eight lanes of a 128-byte store then hit different banks
+        const bool swap = CH == 4 && (c & 2);
+        const uint32_t tile_at = chunk_at<L::kPanel>(tk0, 4 * c + (swap ? 2 : 0));
         auto store = [&](uint32_t dst, const uint4 (&w)[N], const unsigned short (&sc)[N]) {
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const int id = r + 128 * i, tk = id / CH, c = id % CH;
                 const __half2 s2 = __half2half2(__ushort_as_half(sc[i]));
-                uint32_t word[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-                // the upper chunks of a row take their words in the order 2 3 0 1:
-                // the eight lanes of a 128-byte store then hit different banks
-                const bool swap = CH == 4 && (c & 2);
-                if (swap) {
-                    uint32_t t = word[0];
-                    word[0] = word[2], word[2] = t;
-                    t = word[1];
-                    word[1] = word[3], word[3] = t;
-                }
+                const uint32_t word[4] = {swap ? w[i].z : w[i].x, swap ? w[i].w : w[i].y, swap ? w[i].x : w[i].z,
+                                          swap ? w[i].y : w[i].w};
+                const uint32_t at = dst + tile_at + i * (128 / CH * 128);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
                     __half2 v[4];
                     unpack_int(word[x], v);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) v[e] = __hmul2(v[e], s2);
-                    st16(dst + chunk_at<L::kPanel>(tk, 4 * c + (x ^ (swap ? 2 : 0))), as_u32(v[0]), as_u32(v[1]),
-                         as_u32(v[2]), as_u32(v[3]));
+                    // (x only flips bits of the chunk's place in its row, swizzled or not)
+                    st16(at ^ (x << 4), as_u32(v[0]), as_u32(v[1]), as_u32(v[2]), as_u32(v[3]));
                 }
             }
         };
+        rows_of(0);
         load(0, true);
         load(0, false);
         bool ok = true;
@@ -536,6 +543,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             store(smem_u32(smem + L::kK + st * L::kTile), kc, ks);
             fence_async_smem();
             mbar_arrive(&k_full[st]);
+            rows_of(j + 1);
             load(j + 1, true);
             if (turn > 0) ok = __all_sync(0xffffffffu, wait(&v_empty[st], (turn - 1) & 1));
             if (!ok) break;
