@@ -559,3 +559,30 @@ def test_refusals():
             bad()
     torch.cuda.synchronize()
     assert device_error() == 0
+
+
+def test_example_layer_decodes_over_what_it_cached():
+    """examples/kv_cache_decode.py: the last captured step's attention against
+    the oracle on the values that the cache holds."""
+    import os
+    import sys
+
+    from conftest import ROOT
+    from openquant_b200.kv_cache import KVBatch
+
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import kv_cache_decode as ex
+
+    layer, batch, _ = ex.run(requests=3, prompt=50, steps=5, heads=6, kv_heads=2, head_dim=64, page_size=16)
+    q, y = layer.last
+    lengths = batch.lengths.tolist()
+    starts = torch.tensor([0, *np.cumsum(lengths)], dtype=torch.int32).cuda()
+    whole = KVBatch(batch.page_table, batch.lengths, starts, max_tokens=max(lengths))
+    k, v = (f64(x) for x in layer.cache.read(whole, sum(lengths)))
+    for b, n in enumerate(lengths):
+        s = slice(int(starts[b]), int(starts[b + 1]))
+        ref, _, spread, size, mass = ko.attention(f64(q[b:b + 1]), k[s], v[s], 64**-0.5, 1)
+        tol = (np.maximum(2.0**-11 * np.abs(ref), TINY[torch.float16]) + (2.0**-11 + 2.0**-15 * size[..., None]) * spread
+               + 2.0**-31 * mass)
+        assert (np.abs(f64(y[b:b + 1]) - ref) <= tol).all()
+    assert device_error() == 0
