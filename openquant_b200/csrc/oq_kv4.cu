@@ -233,10 +233,14 @@ __device__ __forceinline__ void rotate8(const Rotary &r, const Turn &t, const T 
 // HBM bound: every element is read and written once and needs 3 flops.  A
 // lane owns eight consecutive elements of a head (16 bytes of a 16-bit type),
 // head_dim / 8 lanes a head; a round is the 32 * 8 / head_dim heads that a
-// warp takes at once.  A warp walks rounds of ONE token, kRows at a time with
-// the next kRows in flight: the token's cos and sin are loaded once into
-// registers for all of them, and the partner of an element comes from another
-// lane by shuffle (half layout) or is the lane's own neighbour (interleaved).
+// warp takes at once.  A warp walks rounds of ONE token with kRows of them in
+// flight: the token's cos and sin are loaded once into registers for all of
+// them, and the partner of an element comes from another lane by shuffle (half
+// layout) or is the lane's own neighbour (interleaved).
+// 8192 tokens x 64 heads x 128, bf16: 45 us, 5.9 TB/s, 92 % of the measured copy
+// rate (69 us with one step of four rounds a warp: each then waits for its
+// position and table row by itself).  2049 x 40 x 128 fp32, 64 of them rotated
+// interleaved: 16 us, 82 %.
 template <typename T, bool VEC, int PAIRS>
 __global__ void __launch_bounds__(kWarps * 32)
 rotary_kernel(Rows x, T *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int heads, int head_dim, Rotary rot,
@@ -354,6 +358,12 @@ __device__ __forceinline__ float scale_of(float mx) {
 // and value heads in pairs (k0 v0 k1 v1 ...), so that a key and the value that
 // goes with it sit in neighbouring lane groups of one round.  A group's
 // maximum is a shuffle over group / 8 lanes; a lane's eight codes are one word.
+// 7622 tokens of 32 query and 32 key heads x 128, fp16, rotated: 90 us against
+// 44 us of HBM time.  ncu: issue 64 %, 158 instructions a round of two heads,
+// DRAM 36 % -- instruction-bound: two roundings and a shuffle an element for the
+// rotation, six operations an element for the codes.  (It took 300 us with the
+// queries', keys' and values' rows in one loop, a maximum that propagates NaN
+// by comparisons, and a division per element near a tie of 0.1 %.)
 struct AppendArgs {
     Rows q, k, v;
     void *q_out;
@@ -480,7 +490,8 @@ __global__ void __launch_bounds__(kWarps * 32, VEC && PAIRS != kAny ? 6 : 1) app
 
 // --------------------------------------------------------------- read ----
 //
-// HBM bound; the walk of the append kernel over the key and value heads.
+// HBM bound; the walk of the append kernel over the key and value heads.  7622
+// tokens of 32 heads x 128 to fp16: 30 us against 24 us of HBM time.
 template <typename T>
 __device__ __forceinline__ void values8(uint32_t word, __half scale, T (&o)[8]) {
     __half2 v[4];

@@ -4,7 +4,7 @@
 // Mathematics.  A CTA has 256 query rows of one key head -- rows are (token,
 // query head of the key head) in that order, so all query heads that share a
 // key head share its dequantization -- as two tiles of 128, and walks the
-// cache in blocks of 64 tokens:
+// cache in blocks of 128 tokens:
 //     S = Q K^T (fp32 in TMEM),  p = 2^(S f - m),  O = O + P V
 // with the running maximum m of a row raised only when a score passes it by
 // 2^14 (see kRaise): then O, in TMEM, is multiplied by 2^(m_old - m_new);
@@ -14,10 +14,27 @@
 // A operand.  Queries are fp16 (bf16 rows times a power of two).
 //
 // Roles: warps 0-3 and 4-7 are the softmax of the two tiles (a thread a row),
-// warps 8-11 turn codes into fp16 tiles, one thread of warp 12 issues the
-// products.  Each tile has two S buffers: the scores of a block are computed
-// two blocks ahead of its P V, so a softmax warp finds its next scores ready
-// and the products run while it works.
+// warps 8-11 turn codes into fp16 tiles, warp 12 issues the products.  While
+// one tile's softmax runs, the other tile's products do: P0 V, Q0 K', P1 V,
+// Q1 K', ...  The first half of a P is multiplied while the second is made.
+//
+// What bounds it.  For 4096 queries over 32768 tokens (64 query and 8 key
+// heads, bf16): 3.11 ms, 1.32 PFLOP/s, 80 % of the measured dense bf16 rate,
+// tensor pipe busy 64 % of the cycles.  A block of 256 rows costs about 3400
+// cycles; the products alone take 2048 (64 cycles each, measured with
+// everything else left out), the exponentials 2048 of the 16 a cycle that an
+// SM makes, the operands and the dequantized tiles 2048 of shared memory: the
+// three have to overlap through one S and one P per tile (512 TMEM columns:
+// two S, two O).  Tried against that, and slower: blocks of 64 tokens with two
+// S buffers a tile (the 64-column product reads Q too often, 48 cycles for 32:
+// 5200 cycles for 128 tokens), eight dequantizing warps with S read twice for
+// want of registers (4.1 ms), seven of them, three on V (3.4 ms), and CTAs that
+// stay and fetch the next item's queries early, their items drawn from a
+// counter (3.2 ms, but ragged prompts 198 us for 179 and a mixed step 352 us
+// for 325).  What helped is noted where it is.
+//
+// At short contexts an item's own costs count: 1.7 us to find it and allocate
+// TMEM, 3 us for the queries, 2.5 us for the output.
 //
 // Layouts: Q and K tiles are K-major, 128-byte swizzled, 64 elements a panel;
 // V tiles have the same bytes (row = token) read as an MN-major operand.
@@ -31,15 +48,17 @@ namespace kv4 {
 namespace {
 
 constexpr int kThreads = 512;
-constexpr int kTok = 128;   // cached tokens of a block
-constexpr int kLeastBlocks = 3;  // of a part
-constexpr int kStages = 2;  // K and V tiles in shared memory
+constexpr int kTok = 128;        // cached tokens of a block
+constexpr int kStages = 2;       // K tiles, and V tiles, in shared memory
+constexpr int kLeastBlocks = 3;  // of a part of an item
 constexpr uint32_t kTmemCols = 512;
-// TMEM columns: S buffers (tile, block & 1) of kTok at 0, O tiles at 256 and 256 + head_dim
+// TMEM columns: the tiles' S (and P, in its first half) at 0 and 128, their O at 256 and 256 + head_dim
 constexpr uint32_t kS = 0, kO = 256;
 // Registers a thread: all warps start with kLaunchRegs; the dequantizing and
 // the issuing warpgroup give some up (dec, never above what they have), the
-// softmax warpgroups take them (inc, never below).
+// softmax warpgroups take them (inc, never below): a row of S is 128 of them.
+// (With 184 and stores of 32 registers at a time the rows spilled: 5.1 ms
+// where this takes 3.2.)
 constexpr int kLaunchRegs = 65536 / kThreads, kSoftmaxRegs = 192, kDequantRegs = 88, kIssueRegs = 40;
 static_assert(2 * kSoftmaxRegs + kDequantRegs + kIssueRegs <= 4 * kLaunchRegs, "register split");
 static_assert(kSoftmaxRegs >= kLaunchRegs && kDequantRegs <= kLaunchRegs && kIssueRegs <= kLaunchRegs, "");
@@ -76,13 +95,17 @@ __device__ __forceinline__ void regs_dec() {
 
 // One lane of a converged warp, in a form in which the compiler knows that the
 // warp is converged: it then keeps the products' operands in uniform registers.
+// (Issued behind `lane == 0` a product took 115 cycles instead of 89, in a
+// block that needs 48 of them.)
 __device__ __forceinline__ bool elect_one() {
     uint32_t v;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(v));
     return v != 0;
 }
 
-// 16 bytes that are read once: no line of the (small) L1 is taken for them.
+// 16 bytes that are read once: no line of the L1 is taken for them (beside
+// 198 KB of shared memory it is small: with plain loads an item's queries took
+// 10 us, so 3).
 __device__ __forceinline__ uint4 ld16_once(const void *p) {
     uint4 v;
     asm volatile("ld.global.nc.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -196,12 +219,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t *smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
     uint64_t *bars = reinterpret_cast<uint64_t *>(smem + L::kBars);
-    // s_full, p_full: [tile][block & 1]; pv_done: [tile]
-    uint64_t *q_full = bars, *done = bars + 1, *pv_done = bars + 2, *s_full = bars + 4, *p_full = bars + 8,
-             *k_full = bars + 12, *k_empty = k_full + kStages, *v_full = k_empty + kStages,
-             *v_empty = v_full + kStages;
+    // s_full: [tile]; p_full: [tile][half]; K and V: [stage]
+    uint64_t *q_full = bars, *done = bars + 1, *s_full = bars + 2, *p_full = bars + 4, *k_full = bars + 8,
+             *k_empty = k_full + kStages, *v_full = k_empty + kStages, *v_empty = v_full + kStages;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(v_empty + kStages);
-    static_assert((12 + 4 * kStages) * 8 + 4 <= 256, "barrier space");
+    static_assert((8 + 4 * kStages) * 8 + 4 <= 256, "barrier space");
     const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
 
     asm volatile("griddepcontrol.launch_dependents;");  // the streaming kernel fills the SMs that run out of items
@@ -219,12 +241,11 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 
     if (tid == 0) {
         mbar_init(q_full, 128 * tiles);
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 128);
+            mbar_init(&p_full[2 * i], 128);
+            mbar_init(&p_full[2 * i + 1], 128);
         }
-        mbar_init(&pv_done[0], 1);
-        mbar_init(&pv_done[1], 1);
         for (int i = 0; i < kStages; ++i) {
             mbar_init(&k_full[i], 128);
             mbar_init(&v_full[i], 128);
@@ -264,47 +285,43 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 // rows a load, all in flight.
                 const uint32_t dst = smem_u32(smem + L::kQ + wg * L::kQTile);
                 constexpr int U = 32 / PER;
-                {
-                    uint4 raw[U];
+                uint4 raw[U];
 #pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        const int n = i * PER + sub;
-                        const int64_t from = __shfl_sync(0xffffffffu, (long long)q_at, n);
-                        if (n < live) {
-                            const T *src = static_cast<const T *>(a.q) + from + 8 * c;
-                            if (a.vec) {
-                                raw[i] = ld16_once(src);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&raw[i])[e] = src[e];
-                            }
+                for (int i = 0; i < U; ++i) {
+                    const int n = i * PER + sub;
+                    const int64_t from = __shfl_sync(0xffffffffu, (long long)q_at, n);
+                    raw[i] = make_uint4(0, 0, 0, 0);
+                    if (n < live) {
+                        const T *src = static_cast<const T *>(a.q) + from + 8 * c;
+                        if (a.vec) {
+                            raw[i] = ld16_once(src);
                         } else {
-                            raw[i] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) reinterpret_cast<T *>(&raw[i])[e] = src[e];
                         }
                     }
+                }
 #pragma unroll
-                    for (int i = 0; i < U; ++i) {
-                        const int x = i * PER;  // the warp's rows x .. x + PER
-                        float top = 0.0f, down, v[8];
+                for (int i = 0; i < U; ++i) {
+                    float top = 0.0f, down, v[8];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) v[e] = Elem<T>::to_f32(reinterpret_cast<const T *>(&raw[i])[e]);
-                        if (!std::is_same<T, __half>::value) {
+                    for (int e = 0; e < 8; ++e) v[e] = Elem<T>::to_f32(reinterpret_cast<const T *>(&raw[i])[e]);
+                    if (!std::is_same<T, __half>::value) {
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
+                        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(v[e]));
 #pragma unroll
-                            for (int d = 1; d < LPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                        }
-                        float up = fp16_power<T>(top, down);
-                        if (a.f < 0.0f) up = -up;
-                        if (!std::is_same<T, __half>::value) {  // to the thread that has the row
-                            down = __shfl_sync(0xffffffffu, down, lane % PER * LPR);
-                            if (lane / PER * PER == x) f *= down;
-                        }
-                        uint32_t w[4];
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up));
-                        st16(dst + chunk_at<L::kQPanel>((warp & 3) * 32 + x + sub, c), w[0], w[1], w[2], w[3]);
+                        for (int d = 1; d < LPR; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
                     }
+                    float up = fp16_power<T>(top, down);
+                    if (a.f < 0.0f) up = -up;
+                    if (!std::is_same<T, __half>::value) {  // to the thread that has the row
+                        down = __shfl_sync(0xffffffffu, down, lane % PER * LPR);
+                        if (lane / PER == i) f *= down;
+                    }
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = as_u32(__floats2half2_rn(v[e] * up, v[e + 4] * up));
+                    st16(dst + chunk_at<L::kQPanel>((warp & 3) * 32 + i * PER + sub, c), w[0], w[1], w[2], w[3]);
                 }
                 fence_async_smem();
                 mbar_arrive(q_full);
@@ -476,7 +493,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             }
         };
         uint4 kc[N], vc[N];
-        unsigned short ks[N], vs[N];  // their scales (nothing is done with what is in flight)
+        // Their scales, apart: whatever is done with a value in flight waits for it (packing
+        // the two of a chunk into one register cost 1000 cycles a block).
+        unsigned short ks[N], vs[N];
         // Chunk i of the thread: token r / CH + i * 128 / CH, 16-byte chunk r % CH, so
         // that all of them have one place within 16 tokens and one swizzle.
         const int tk0 = r / CH, c = r % CH;
@@ -484,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
         const uint8_t *k_lane = a.k_codes + code_at, *v_lane = a.v_codes + code_at;
         const unsigned short *ks_lane = reinterpret_cast<const unsigned short *>(a.k_scales) + scale_at;
         const unsigned short *vs_lane = reinterpret_cast<const unsigned short *>(a.v_scales) + scale_at;
-        uint32_t r16[N];  // the chunks' rows / 16 in the cache, of block `at_block`
+        uint32_t r16[N];  // the chunks' rows / 16 in the cache, of the block that is loaded
         auto rows_of = [&](int j) {
             if (j >= nblk) return;
             if (j % kAhead == 0) look_up(j);
@@ -610,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     }
                 }
             }
-            // Every product this thread issued has completed once `done` fires.
+            // Every product this warp issued has completed once `done` fires.
             if (elect_one()) tc_commit(done);
             __syncwarp();
             wait(done, 0);
@@ -626,7 +645,6 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
 // Adds the parts of the items that were cut: a thread a row, 16 columns a CTA.
 template <typename T, int HD>
 __global__ void __launch_bounds__(kPromptRows) join_prompt_kernel(const __grid_constant__ AttnArgs a, int cuts) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
     Item it;
     if (!find_item<kPromptRows>(a, blockIdx.x, cuts, it) || it.parts == 1) return;
     const int r = threadIdx.x, row = it.row0 + r;
