@@ -33,6 +33,12 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 4;   // warps a CTA; each works by itself
+// CTAs a SM: three leave 168 registers a thread.  With four, 128, the loop
+// spills: 64 ragged sequences 86 us for 83.  Two tiles of columns of head_dim
+// 128 hold 64 more sums and need two CTAs: 16 rows on 16 x 8000 tokens 62 us for
+// 66, on 8 x 4000 tokens of 32 key heads 62 for 65.
+template <int HD, int NT>
+constexpr int kCtas = NT == 2 && HD == 128 ? 2 : 3;
 constexpr int kStages = 4;  // 16-token stages of a warp, in use or in flight
 // Cost of beginning an item and the smallest share of a warp, in blocks of 16
 // tokens.  Measured with 2, 6, 12 and 4 .. 40: 64 ragged sequences 91 / 87 / 86
@@ -139,6 +145,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with a zero accumulator to begin with (no registers to clear).
+__device__ __forceinline__ void mma16816_first(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -172,7 +186,7 @@ __device__ __forceinline__ void write_slice(const Args &a, const Work &w, int he
 // are staged 16 bytes longer than they are, which makes both the ldmatrix of
 // the keys and the 4- or 8-byte reads of the values free of bank conflicts.
 template <typename T, int HD, int GS, int NT>
-__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(const Args a) {
+__global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(const Args a) {
     using S = Shape<HD, NT>;
     constexpr int kCols = S::kCols, kPitch = S::kPitch;
     constexpr int NG = HD / GS;             // groups a row
@@ -180,7 +194,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
     constexpr int kCodes = 16 * kPitch;     // staged codes of 16 tokens
     constexpr int kScales = 16 * NG * 2;
     constexpr int kStage = 2 * kCodes + 2 * kScales;
-    constexpr int H = NT == 1 ? 2 : 1;      // blocks a step: one has two chains of products with NT = 2
+    // blocks a step, for two chains of products to overlap; with NT = 2 too (16
+    // rows on 16 x 8000 tokens 59.6 us, 62.3 with one block)
+    constexpr int H = 2;
     constexpr int kSteps = kStages / H;     // steps in flight or in use
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -354,10 +370,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
             for (int h = 0; h < H; ++h) {
                 const unsigned char *st = ring + ((i + h) % kStages) * kStage;
                 const uint32_t su = ring_u + ((i + h) % kStages) * kStage;
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) s[h][j][e] = 0.0f;
                 uint32_t kw[2][CH];  // words t4 of each chunk of rows g, g + 8
                 if (CH == 4) {
                     // matrix i of the four: chunk i of rows 0..7
@@ -394,10 +406,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                 for (int G = 0; G < NG; ++G) {
                     float acc[NT][4];
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) acc[j][e] = 0.0f;
-#pragma unroll
                     for (int cc = 0; cc < GS / 32; ++cc) {
                         const int c = G * (GS / 32) + cc;
                         __half2 x0[4], x1[4];
@@ -405,20 +413,24 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 4 : 3) stream_kernel(co
                         unpack_int(kw[1][c], x1);
 #pragma unroll
                         for (int j = 0; j < NT; ++j) {
-                            mma16816(acc[j], as_u32(x0[0]), as_u32(x1[0]), as_u32(x0[1]), as_u32(x1[1]), qf[j][c][0],
-                                     qf[j][c][1]);
+                            if (cc == 0)
+                                mma16816_first(acc[j], as_u32(x0[0]), as_u32(x1[0]), as_u32(x0[1]), as_u32(x1[1]),
+                                               qf[j][c][0], qf[j][c][1]);
+                            else
+                                mma16816(acc[j], as_u32(x0[0]), as_u32(x1[0]), as_u32(x0[1]), as_u32(x1[1]),
+                                         qf[j][c][0], qf[j][c][1]);
                             mma16816(acc[j], as_u32(x0[2]), as_u32(x1[2]), as_u32(x0[3]), as_u32(x1[3]), qf[j][c][2],
                                      qf[j][c][3]);
                         }
                     }
                     const float s0 = __half2float(ks[0][G]), s1 = __half2float(ks[1][G]);
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        s[h][j][0] = fmaf(s0, acc[j][0], s[h][j][0]);
-                        s[h][j][1] = fmaf(s0, acc[j][1], s[h][j][1]);
-                        s[h][j][2] = fmaf(s1, acc[j][2], s[h][j][2]);
-                        s[h][j][3] = fmaf(s1, acc[j][3], s[h][j][3]);
-                    }
+                    for (int j = 0; j < NT; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float sc = e < 2 ? s0 : s1;
+                            s[h][j][e] = G == 0 ? sc * acc[j][e] : fmaf(sc, acc[j][e], s[h][j][e]);
+                        }
                 }
             }
 
@@ -687,8 +699,13 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
 }
 
 // CTAs of the streaming kernel: what fits on the GPU at once.
-template <int NT>
-int share_of() { return sm_count() * (NT == 1 ? 4 : 3); }
+template <int HD, int NT>
+int share_of() { return sm_count() * kCtas<HD, NT>; }
+
+int share_of(const oq_kv4_cache *c, int nt) {
+    if (c->head_dim == 64) return nt == 1 ? share_of<64, 1>() : share_of<64, 2>();
+    return nt == 1 ? share_of<128, 1>() : share_of<128, 2>();
+}
 
 template <int HD, int GS>
 constexpr size_t ring_bytes() {
@@ -712,7 +729,7 @@ int columns_of(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
 
 template <typename T, int HD, int GS, int NT>
 int stream_launch(Args &a, const oq_kv4_batch *batch, bool beside, cudaStream_t st) {
-    const int share = share_of<NT>();
+    const int share = share_of<HD, NT>();
     auto kern = stream_kernel<T, HD, GS, NT>;
     const size_t smem = ring_bytes<HD, GS>() + (batch->sequences + 1) * 8;  // the prefix follows the rings
     if (int rc = allow_dynamic_smem(reinterpret_cast<const void *>(kern), smem)) return rc;
@@ -770,7 +787,7 @@ int attention_typed(Args &a, const oq_kv4_cache *c, const oq_kv4_batch *batch, i
 // Workspace of the streaming kernel.
 int64_t stream_bytes(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
     const int nt = columns_of(c, b, q_heads);
-    const int64_t warps = (nt == 1 ? share_of<1>() : share_of<2>()) * kWarps;
+    const int64_t warps = (int64_t)share_of(c, nt) * kWarps;
     return warps * 2 * (16 * nt + nt * c->head_dim * 8) * 4;
 }
 
