@@ -19,13 +19,16 @@
 //
 // What bounds it.  The cache has to be read once: 144 bytes a token and key
 // head (head_dim 128, groups of 32).  64 ragged sequences of 333 to 8192 tokens
-// (64 query, 8 key heads): 86 us, 57 % of the measured copy rate, DRAM traffic
-// 1.01 x the cache's bytes; two of 100003 and 131071 tokens (groups of 64) 69
-// us, 56 %.  ncu: instruction issue 62 % of the cycles with 16 warps an SM,
-// 23 instructions a token and key head, most of them the unpacking (9 for eight
+// (64 query, 8 key heads): 81.5 us, 60 % of the measured copy rate, DRAM traffic
+// 1.00 x the cache's bytes; two of 100003 and 131071 tokens (groups of 64) 65
+// us, 60 %.  ncu: instruction issue 61 % of the cycles with 12 warps an SM, 22
+// instructions a token and key head, most of them the unpacking (9 for eight
 // codes, and 4 more for the scale of V); no bank conflicts, tensor pipe 22 %.
-// So it is bound by issue and by the latency of what each warp does in turn;
-// 20 warps an SM need 96 registers and spill (117 us).
+// So it is bound by issue and by the latency of what each warp does in turn.
+// Fewer warps are slower (8 an SM: 122 us) and more do not have the registers
+// (16: 88 us with one block a step, 86 us with two and spills; 20: 117 us).
+// Deeper rings (6 stages: 82.8 us) and scores computed a step ahead (85 us) cost
+// more than they hide.
 #include "oq_kv4_attention.cuh"
 
 namespace oq {
@@ -33,7 +36,7 @@ namespace kv4 {
 namespace {
 
 constexpr int kWarps = 4;   // warps a CTA; each works by itself
-// CTAs a SM: three leave 168 registers a thread.  With four, 128, the loop
+// CTAs an SM: three leave 168 registers a thread.  With four, 128, the loop
 // spills: 64 ragged sequences 86 us for 83.  Two tiles of columns of head_dim
 // 128 hold 64 more sums and need two CTAs: 16 rows on 16 x 8000 tokens 62 us for
 // 66, on 8 x 4000 tokens of 32 key heads 62 for 65.
@@ -41,8 +44,8 @@ template <int HD, int NT>
 constexpr int kCtas = NT == 2 && HD == 128 ? 2 : 3;
 constexpr int kStages = 4;  // 16-token stages of a warp, in use or in flight
 // Cost of beginning an item and the smallest share of a warp, in blocks of 16
-// tokens.  Measured with 2, 6, 12 and 4 .. 40: 64 ragged sequences 91 / 87 / 86
-// us for the first; one sequence of 1000 tokens and 32 key heads 12 us with a
+// tokens.  Measured with 8, 12, 14 and 4 .. 40: 64 ragged sequences 83.2 / 81.6 /
+// 82.2 us for the first; one sequence of 1000 tokens and 32 key heads 12 us with a
 // least share of 4, 29 us with 40.
 constexpr int kSetup = 12, kLeast = 4;
 
@@ -181,10 +184,10 @@ __device__ __forceinline__ void write_slice(const Args &a, const Work &w, int he
 // other: ragged lengths load the warps alike, and no warp waits for another.
 // A share begins and ends inside an item, whose parts the joining kernel adds
 // in a fixed order.  A warp streams its blocks through its own ring of cp.async
-// stages, two blocks at a time (two independent chains of products) or, with two
-// column tiles, one; the rows
-// are staged 16 bytes longer than they are, which makes both the ldmatrix of
-// the keys and the 4- or 8-byte reads of the values free of bank conflicts.
+// stages, two blocks at a time (two independent chains of products; with one,
+// 16 rows on 16 x 8000 tokens take 62.3 us for 59.6).  Rows are staged 16 bytes
+// longer than they are, which makes both the ldmatrix of the keys and the 4- or
+// 8-byte reads of the values free of bank conflicts.
 template <typename T, int HD, int GS, int NT>
 __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(const Args a) {
     using S = Shape<HD, NT>;
@@ -194,9 +197,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
     constexpr int kCodes = 16 * kPitch;     // staged codes of 16 tokens
     constexpr int kScales = 16 * NG * 2;
     constexpr int kStage = 2 * kCodes + 2 * kScales;
-    // blocks a step, for two chains of products to overlap; with NT = 2 too (16
-    // rows on 16 x 8000 tokens 59.6 us, 62.3 with one block)
-    constexpr int H = 2;
+    constexpr int H = 2;                    // blocks a step
     constexpr int kSteps = kStages / H;     // steps in flight or in use
     extern __shared__ __align__(16) unsigned char smem[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -275,10 +276,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                     rows16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * pp + (blk - pg * pp));
             }
         };
-        auto load = [&](int i) {
+        auto load = [&](int i, int at) {  // block i, staged at byte `at` of the ring
             if (i < nblk) {
                 const uint32_t r16 = __shfl_sync(0xffffffffu, rows16, i & 31);
-                const uint32_t dst = ring_u + (i % kStages) * kStage;
+                const uint32_t dst = ring_u + at;
 #pragma unroll
                 for (int j = 0; j < HD / 64; ++j) {
                     cp16(dst + to_codes + j * (32 / CH * kPitch), k_lane + (size_t)r16 * (16 * HD / 2) + j * 512);
@@ -292,7 +293,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
         __syncwarp();  // the ring's last reads (of the item before) are done
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
-            load(i);
+            load(i, i * kStage);
             if ((i + 1) % H == 0) cp_commit();
         }
 
@@ -359,6 +360,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             l[j][0] = l[j][1] = 0.0f;
         }
 
+        int at = 0;  // byte of the step in the ring
         for (int i = 0; i < nblk; i += H) {
             cp_wait<kSteps - 1>();
             __syncwarp();
@@ -368,8 +370,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             float s[H][NT][4];
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const unsigned char *st = ring + ((i + h) % kStages) * kStage;
-                const uint32_t su = ring_u + ((i + h) % kStages) * kStage;
+                const unsigned char *st = ring + at + h * kStage;
+                const uint32_t su = ring_u + at + h * kStage;
                 uint32_t kw[2][CH];  // words t4 of each chunk of rows g, g + 8
                 if (CH == 4) {
                     // matrix i of the four: chunk i of rows 0..7
@@ -497,7 +499,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             // ---- o += V^T p: rows d = HD/8 g + ..., tokens 2 t4, +1, +8, +9
 #pragma unroll
             for (int h = 0; h < H; ++h) {
-                const unsigned char *vc = ring + ((i + h) % kStages) * kStage + kCodes;
+                const unsigned char *vc = ring + at + h * kStage + kCodes;
                 const __half *vsc = reinterpret_cast<const __half *>(vc + kCodes + kScales);
                 constexpr int W = HD / 64;  // words a lane takes of a token
                 const int G = NG == 1 ? 0 : (HD / 8 * g) / GS;
@@ -551,8 +553,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             // later blocks take the place of these
             if (((i + kStages) & 31) == 0) look_up(i + kStages);
 #pragma unroll
-            for (int h = 0; h < H; ++h) load(i + kStages + h);
+            for (int h = 0; h < H; ++h) load(i + kStages + h, at + h * kStage);
             cp_commit();
+            at = at + H * kStage < kStages * kStage ? at + H * kStage : 0;
         }
         cp_wait<0>();
 
@@ -716,8 +719,9 @@ constexpr size_t ring_bytes() {
 // 16 rows, each of which reads the cache again, from L2), the others go to the
 // prompt kernel, whose tiles have 128 rows.  Single tokens are always streamed.
 // Measured, streamed / prompt kernel: head_dim 64, 37 rows over 23 x 11139
-// tokens 173 / 186 us, 48 rows over 34 x 8902..17804 tokens 52 / 62 us; head_dim
-// 128, 40 rows over 16 x 8000 tokens 154 / 122 us, 64 rows 198 / 123 us.
+// tokens 160 / 185 us, 48 rows over 34 x 8902..17804 tokens 50 / 62 us; head_dim
+// 128, 40 rows over 16 x 8000 tokens 142 / 112 us, 64 rows 186 / 113 us (32 rows,
+// streamed, 99 us).
 int few_rows(const oq_kv4_cache *c, int q_heads) {
     const int ratio = q_heads / c->kv_heads, few = c->head_dim == 64 ? 64 : 32;
     return ratio > few ? ratio : few;
