@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import threading
 
 import torch
 
@@ -38,7 +39,7 @@ _CODES = {torch.float32: nat.OQ_F32, torch.float16: nat.OQ_F16, torch.bfloat16: 
 _ROTARY_INTERLEAVED, _ROTARY_INVERSE = 1, 2
 _NOT_CAUSAL = 1
 MAX_SEQUENCES = 2048
-_KEEP_BYTES, _KEEP_STREAMS = 32 << 20, 4  # workspaces that a KVBatch keeps
+_KEEP_BYTES, _KEEP_BUFFERS = 32 << 20, 4  # workspaces that a KVBatch keeps
 
 
 # -------------------------------------------------------------- rotary --
@@ -262,21 +263,23 @@ class KVBatch:
                          n, int(page_table.shape[1]), max_tokens)
         self._ref = ctypes.byref(self._c)
         self._ws = {}  # (cache shape, q_heads, tokens) -> workspace bytes
-        self._buffers = {}  # stream -> workspace
-
+        self._buffers = {}  # (stream, host thread) -> workspace
 
     def _workspace(self, nbytes, device):
-        """nbytes of scratch memory for a call on the current stream: one buffer
-        per stream, as calls on one stream follow each other; a captured call
-        has its own from the graph's pool, and large ones are not kept."""
+        """nbytes of scratch memory for a call on the current stream.  A call is
+        several kernels that hand results on through it: one buffer per stream
+        and host thread, as only the launches of one thread on one stream are
+        sure to follow each other call by call (two threads on the stream that
+        they share by default may launch theirs in turn).  A captured call has
+        its own from the graph's pool, and large ones are not kept."""
         if nbytes > _KEEP_BYTES or torch.cuda.is_current_stream_capturing():
             return torch.empty(nbytes, dtype=torch.uint8, device=device)
-        stream = _stream_handle(self._dev)
-        buf = self._buffers.get(stream)
+        key = (_stream_handle(self._dev), threading.get_ident())
+        buf = self._buffers.get(key)
         if buf is None or buf.numel() < nbytes:
-            if len(self._buffers) >= _KEEP_STREAMS:
+            if len(self._buffers) >= _KEEP_BUFFERS:
                 self._buffers.clear()
-            buf = self._buffers[stream] = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            buf = self._buffers[key] = torch.empty(nbytes, dtype=torch.uint8, device=device)
         return buf
 
 
