@@ -76,7 +76,8 @@ def _frequencies(dim, base, scaling):
     def index(n):
         return dim * math.log(original / (n * 2 * math.pi)) / (2 * math.log(base))
 
-    first, last = max(math.floor(index(high)), 0), min(math.ceil(index(low)), dim // 2 - 1)
+    # either pair may lie outside the head: the line goes through it all the same
+    first, last = math.floor(index(high)), math.ceil(index(low))
     ramp = ((torch.arange(dim // 2, dtype=torch.float64) - first) / max(last - first, 1e-3)).clamp(0, 1)
     size = float(scaling.get("magnitude", 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
     return freq * (1 - ramp) + freq / factor * ramp, size
@@ -94,7 +95,9 @@ def rotary_table(positions, rotary_dim, *, base=10000.0, scaling=None, device=No
       {"type": "parts", "factor": f, "original_positions": n, "low": 1, "high": 32,
        "magnitude": ...}                pairs that turn more than `high` times over n positions keep
                                         their angle, those below `low` turns have it divided by f, linear
-                                        in the pair's index between; cos and sin times magnitude
+                                        in the pair's index between (from the last whole index that
+                                        turns at least `high` times to the first that turns at most `low`
+                                        times, in the head or outside it); cos and sin times magnitude
                                         (0.1 ln f + 1)
       {"type": "smooth", "factor": f, "original_positions": n, "low": 1, "high": 4}
                                         the same with a passage linear in the number of turns

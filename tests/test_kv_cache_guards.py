@@ -1,7 +1,9 @@
 """4-bit key/value cache: calls at the edge of what is allowed, as far as that
 needs no GPU."""
+import math
 import threading
 
+import pytest
 import torch
 
 
@@ -41,3 +43,31 @@ def test_workspaces_of_many_threads_are_not_all_kept(monkeypatch):
         monkeypatch.setattr(threading, "get_ident", lambda i=i: i)
         assert batch._workspace(64, "cpu").numel() == 64
     assert len(batch._buffers) <= 4
+
+
+@pytest.mark.parametrize("dim, base, original, factor", [
+    (128, 1e4, 4096, 8.0),     # both turning points among the pairs
+    (128, 1e4, 131072, 4.0),   # even the slowest pair turns more than once
+    (32, 1e4, 131072, 8.0),
+    (64, 500.0, 65536, 2.0),
+    (128, 1e4, 150, 4.0),      # even the fastest pair turns less than 32 times
+    (64, 1e4, 5, 4.0),         # no pair turns once
+])
+def test_rotary_scaling_by_parts_is_a_line_between_the_turning_points(dim, base, original, factor):
+    from openquant_b200.kv_cache import _frequencies
+
+    plain, _ = _frequencies(dim, base, None)
+    got, _ = _frequencies(dim, base, {"type": "parts", "factor": factor, "original_positions": original})
+    turns = original / (2 * math.pi) * base ** (-2.0 * torch.arange(-8 * dim, 9 * dim, dtype=torch.float64) / dim)
+    index = range(-8 * dim, 9 * dim)
+    first = max(i for i, t in zip(index, turns) if t >= 32)
+    last = min(i for i, t in zip(index, turns) if t <= 1)
+    for i in range(dim // 2):
+        share = min(max((i - first) / (last - first), 0.0), 1.0)  # of the divided angle
+        want = plain[i] * (1 - share) + plain[i] / factor * share
+        assert math.isclose(float(got[i]), float(want), rel_tol=1e-12), i
+        t = original * plain[i] / (2 * math.pi)
+        if t >= 32 * base ** (2 / dim):
+            assert got[i] == plain[i]
+        if t <= base ** (-2 / dim):
+            assert math.isclose(float(got[i]), float(plain[i]) / factor, rel_tol=1e-12)
