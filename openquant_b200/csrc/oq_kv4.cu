@@ -294,10 +294,11 @@ __device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, in
     int first, count;
     tokens_of(bt, seq, tokens, first, count);
     if (t < first || t >= first + count) return false;
-    const int p = length_of(bt, seq, page_size) - count + (int)(t - first);
-    pos = p;
-    if (p >= 0) {
-        const int slot = p / page_size, page = __ldg(bt.table + (int64_t)seq * bt.max_pages + slot);
+    // The place that the length gives, inside the page-table row or not: a
+    // length cut to the row would move the tokens onto others that are there.
+    pos = (int64_t)__ldg(bt.lengths + seq) - count + (t - first);
+    if (pos >= 0 && pos < (int64_t)bt.max_pages * page_size) {
+        const int p = (int)pos, slot = p / page_size, page = __ldg(bt.table + (int64_t)seq * bt.max_pages + slot);
         if (page >= 0 && page < pages) at = ((int64_t)page * kv_heads) * page_size + (p - slot * page_size);
     }
     if (at < 0 && (threadIdx.x & 31) == 0) index_error();

@@ -2,10 +2,12 @@
 in test_kv_cache_gpu.py, whose cases these use."""
 import threading
 
+import numpy as np
 import pytest
 import torch
 
-from test_kv_cache_gpu import Case, _device, device_error  # noqa: F401 (_device: a fixture)
+import kv4_oracle as ko
+from test_kv_cache_gpu import Case, _device, device_error, f64  # noqa: F401 (_device: a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +55,45 @@ def test_two_streams_in_flight_at_once():
     torch.cuda.synchronize()
     for ys, y in zip(got, want):
         assert all(torch.equal(x, y) for x in ys)
+
+
+@pytest.mark.parametrize("length, count, kept", [(33, 1, []), (33, 2, [0]), (34, 5, [0, 1, 2]), (1 << 30, 2, []),
+                                                 ((1 << 31) - 1, 3, []), (1, 3, [2]), (-5, 2, []),
+                                                 (-(1 << 31), 3, [])])
+def test_append_beyond_the_page_table(length, count, kept):
+    """Tokens whose place is outside the page table (of 32 here) are left out
+    with an error: none of them lands on a token that is there."""
+    from openquant_b200.kv_cache import Int4KVCache, KVBatch, rotary_table
+
+    dev = dict(dtype=torch.int32, device="cuda")
+    cache = Int4KVCache.allocate(4, 16, 2, 64)
+    k, v = (torch.randn(32, 2, 64, device="cuda").half() for _ in range(2))
+    pages = torch.tensor([[2, 1]], **dev)
+    cache.append(k, v, KVBatch(pages, torch.tensor([32], **dev), torch.tensor([0, 32], **dev), max_tokens=32))
+    arrays = (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)
+    before = [x.clone() for x in arrays]
+    k, v = (torch.randn(count, 2, 64, device="cuda").half() for _ in range(2))
+    q = torch.randn(count, 4, 64, device="cuda").half()
+    table = rotary_table(64, 64)
+    batch = KVBatch(pages, torch.tensor([length], **dev), torch.tensor([0, count], **dev), max_tokens=count)
+    got = cache.append(k, v, batch, q=q, table=table)
+    assert device_error() == 3
+    places = [length - count + i for i in range(count)]
+    assert [i for i, p in enumerate(places) if 0 <= p < 32] == kept
+    want_k = ko.rotate(f64(k).astype(np.float32), table.cpu().numpy(), [p if 0 <= p < 64 else 0 for p in places])
+    want_q = ko.rotate(f64(q).astype(np.float32), table.cpu().numpy(), [p if 0 <= p < 64 else 0 for p in places])
+    held = [ko.quantise(want_k, 32), ko.quantise(f64(v).astype(np.float32), 32)]
+    want = [x.cpu().numpy() for x in before]
+    for i in kept:
+        page, row = [2, 1][places[i] // 16], places[i] % 16
+        for x, (codes, scales) in enumerate(held):
+            want[2 * x][page, :, row], want[2 * x + 1][page, :, row] = ko.pack(codes[i]), scales[i]
+    for x, y in zip(arrays, want):
+        assert np.array_equal(x.cpu().numpy(), y)
+    for i, p in enumerate(places):
+        if 0 <= p < 64:  # queries turn by the same places
+            assert torch.equal(got[i].cpu(), torch.from_numpy(want_q[i]).half())
+    for x, (codes, scales) in zip(cache.read(batch, count), held):
+        for i in range(count):
+            assert np.array_equal(f64(x[i]), ko.values(codes[i], scales[i]) if i in kept else np.zeros((2, 64)))
+    assert device_error() == 3
