@@ -57,10 +57,12 @@ __device__ __forceinline__ void tokens_of(const Batch &bt, int b, int64_t tokens
     count = e - s;
 }
 
-// Length of sequence b, kept inside its page-table row.
-__device__ __forceinline__ int length_of(const Batch &bt, int b, int page_size) {
+// Cached tokens of sequence b that its page-table row has room for; `end`: its
+// length as it is, from which the step's tokens have their positions.
+__device__ __forceinline__ int length_of(const Batch &bt, int b, int page_size, int &end) {
     const int64_t cap = (int64_t)bt.max_pages * page_size;
     const int n = __ldg(bt.lengths + b);
+    end = max(n, 0);
     if (n < 0 || n > cap) {
         index_error();
         return n < 0 ? 0 : (int)cap;

@@ -64,18 +64,21 @@ struct Shape {
 // Work of sequence b: an item per key head and per block of `cols` query
 // rows, of nb blocks of 16 cached tokens (from block b0 on) and kSetup units.
 struct Work {
-    int first, count, rows, length;
-    int floor;  // first cached token any row sees
+    int first, count, rows;
+    int length, base;  // cached tokens that can be read; position of the step's first token
+    int floor;         // first cached token any row sees
     int b0, nb, blocks;
 };
 
 __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
     Work w;
     tokens_of(a.batch, b, a.tokens, w.first, w.count);
-    w.length = length_of(a.batch, b, a.page_size);
+    int end;
+    w.length = length_of(a.batch, b, a.page_size, end);
+    w.base = end - w.count;
     w.rows = w.count * a.ratio;
     w.blocks = w.rows > a.few ? 0 : (w.rows + cols - 1) / cols;
-    w.floor = a.window > 0 ? (int)max((int64_t)w.length - w.count + 1 - a.window, (int64_t)0) : 0;
+    w.floor = a.window > 0 ? (int)max((int64_t)w.base + 1 - a.window, (int64_t)0) : 0;
     w.b0 = w.floor >> 4;
     w.nb = max(((w.length + 15) >> 4) - w.b0, 1);
     return w;
@@ -337,15 +340,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int col = row0 + 8 * j + 2 * t4 + e;
-                pos[j][e] = w.length - w.count + (col < w.rows ? col / a.ratio : w.count - 1);
+                pos[j][e] = w.base + (col < w.rows ? col / a.ratio : w.count - 1);
             }
         }
         // tokens that every column of the item sees
         int all_vis = w.length, all_low = 0;
-        if (a.causal) all_vis = w.length - w.count + row0 / a.ratio + 1;
+        if (a.causal) all_vis = w.base + row0 / a.ratio + 1;
         if (a.window > 0) {
             const int last = min(row0 + kCols, w.rows) - 1;
-            all_low = (int)max((int64_t)w.length - w.count + last / a.ratio + 1 - a.window, (int64_t)0);
+            all_low = (int)max((int64_t)w.base + last / a.ratio + 1 - a.window, (int64_t)0);
         }
 
         float o[NT][HD / 16][4], m[NT][2], l[NT][2], most[NT][2];  // most: the score at which m is raised

@@ -145,7 +145,8 @@ __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint
 
 // What item `id` (over all sequences with more than a.few rows) works on.
 struct Item {
-    int b, first, count, length, rows, head, row0;
+    int b, first, count, rows, head, row0;
+    int length, base;   // cached tokens that can be read; position of the step's first token
     int nblk;       // blocks of kTok cached tokens from `lo` on, for all its parts
     int parts;      // parts it is cut into
     int floor, lo, hi;  // first visible token, the same down to 16, one past the last
@@ -191,15 +192,17 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int id, int cuts, I
     it.b = found[0];
     if (it.b < 0) return false;
     tokens_of(a.batch, it.b, a.tokens, it.first, it.count);
-    it.length = length_of(a.batch, it.b, a.page_size);
+    int end;
+    it.length = length_of(a.batch, it.b, a.page_size, end);
+    it.base = end - it.count;
     it.rows = it.count * a.ratio;
     const int blocks = (it.rows + kPromptRows - 1) / kPromptRows;
     // the last rows see most: they go first
     it.head = found[1] % a.kv_heads;
     it.row0 = (blocks - 1 - found[1] / a.kv_heads) * kPromptRows;
-    const int last = min(it.row0 + kPromptRows, it.rows) - 1, base_pos = it.length - it.count;
-    const int p0 = base_pos + it.row0 / a.ratio, p1 = base_pos + last / a.ratio;
-    it.hi = a.causal ? p1 + 1 : it.length;
+    const int last = min(it.row0 + kPromptRows, it.rows) - 1;
+    const int p0 = it.base + it.row0 / a.ratio, p1 = it.base + last / a.ratio;
+    it.hi = a.causal ? min(p1 + 1, it.length) : it.length;
     it.floor = a.window > 0 ? (int)max((int64_t)p0 + 1 - a.window, (int64_t)0) : 0;
     it.lo = it.floor & ~15;
     it.nblk = it.hi > it.lo ? (it.hi - it.lo + kTok - 1) / kTok : 0;
@@ -232,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
     if (!find_item<kThreads>(a, blockIdx.x / cuts, cuts, it) || part >= it.parts) return;
     const int b = it.b, first = it.first, length = it.length, rows = it.rows, head = it.head, row0 = it.row0;
     const int nrows = min(kPromptRows, rows - row0);
-    const int64_t base = (int64_t)length - it.count;  // position of the step's first token
+    const int base = it.base;
     // this part's blocks
     const int j0 = (int)((int64_t)part * it.nblk / it.parts), j1 = (int)((int64_t)(part + 1) * it.nblk / it.parts);
     const int nblk = j1 - j0;
@@ -327,12 +330,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 mbar_arrive(q_full);
             }
             if (f == 0.0f) f = 1e-30f;  // masked scores are -inf before they are multiplied
-            const int64_t pos = base + tk;
-            const int64_t vis = a.causal ? pos + 1 : length, low = a.window > 0 ? pos + 1 - a.window : 0;
+            // tokens [low, vis) are what the row sees
+            const int vis = a.causal ? min(base + tk + 1, length) : length;
+            const int low = a.window > 0 ? (int)max((int64_t)base + tk + 1 - a.window, (int64_t)0) : 0;
             // tokens that every row of the tile sees
             const int last = min(row0 + wg * 128 + 127, rows - 1);
-            const int64_t all_vis = a.causal ? base + (row0 + wg * 128) / a.ratio + 1 : length;
-            const int64_t all_low = a.window > 0 ? base + last / a.ratio + 1 - a.window : 0;
+            const int all_vis = a.causal ? min(base + (row0 + wg * 128) / a.ratio + 1, length) : length;
+            const int all_low = a.window > 0 ? (int)max((int64_t)base + last / a.ratio + 1 - a.window, (int64_t)0) : 0;
             const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + quarter + kS + wg * kTok, to = tmem + quarter + kO + wg * HD;
             float m = -1e30f;

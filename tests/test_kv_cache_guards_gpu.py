@@ -7,9 +7,28 @@ import pytest
 import torch
 
 import kv4_oracle as ko
-from test_kv_cache_gpu import Case, _device, device_error, f64  # noqa: F401 (_device: a fixture)
+from test_kv_cache_gpu import TINY, U, Case, _device, device_error, f64  # noqa: F401 (_device: a fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+def check_seen(case, q, out, log_sum, seen, scale=None):
+    """Row t of the step against the oracle on the tokens `seen[t]` = (sequence,
+    indices) that it sees."""
+    scale = q.shape[2] ** -0.5 if scale is None else scale
+    held = [(case.sequence(b, 0), case.sequence(b, 1)) for b in range(len(case.lengths))]
+    got, lse = f64(out), f64(log_sum)
+    for t, (b, idx) in enumerate(seen):
+        k, v = (x[idx] for x in held[b])
+        ref, want, spread, size, mass = (x[0] for x in ko.attention(f64(q[t:t + 1]), k, v, scale, 1, causal=False))
+        d = 2.0**-16 * size
+        tol = (np.maximum(U[out.dtype] * np.abs(ref), TINY[out.dtype]) + (2.0**-11 + 2 * d[:, None]) * spread
+               + 2.0**-31 * mass + 1e-30)
+        assert (np.abs(got[t] - ref) <= tol).all(), t
+        if len(idx):
+            assert (np.abs(lse[t] - want) <= d + 2.0**-20 * (1 + np.abs(want))).all(), t
+        else:
+            assert not got[t].any() and (lse[t] == -np.inf).all(), t
 
 
 def test_threads_share_a_batch_and_a_stream():
@@ -97,3 +116,31 @@ def test_append_beyond_the_page_table(length, count, kept):
         for i in range(count):
             assert np.array_equal(f64(x[i]), ko.values(codes[i], scales[i]) if i in kept else np.zeros((2, 64)))
     assert device_error() == 3
+
+
+@pytest.mark.parametrize("dim, heads, counts", [(128, 4, [2, 1, 6]), (64, 8, [9, 1, 60]), (128, 8, [40, 3, 200])])
+@pytest.mark.parametrize("window, causal", [(0, True), (0, False), (13, True), (5, False)])
+def test_attention_beyond_the_page_table(dim, heads, counts, window, causal):
+    """Tokens past the page table are not there; the queries keep the
+    positions that the length gives them."""
+    case = Case([48, 20, 240], counts, 2, dim, page=16, seed=dim, junk=True)
+    over = [53, 20, 241]  # rows of the table for 240 tokens; the first sequence has pages for 48
+    case.batch.page_table[0, 3:] = case.batch.page_table[0, 0]
+    case.batch.lengths.copy_(torch.tensor(over, dtype=torch.int32))
+    table = case.batch.page_table[:, :3].contiguous()
+    from openquant_b200.kv_cache import KVBatch
+
+    q = case.queries(heads, dim, torch.float16)
+    for batch, caps in ((case.batch, [240, 240, 240]), (KVBatch(table, case.batch.lengths, case.batch.starts,
+                                                              max_tokens=max(counts)), [48, 48, 48])):
+        out, lse = case.cache.attention(q, batch, window=window, causal=causal, return_log_sum=True)
+        assert device_error() == 3
+        seen, rows = [], []
+        for b, (n, c, cap) in enumerate(zip(over, counts, caps)):
+            for p in range(n - c, n):
+                hi = min(p + 1, n, cap) if causal else min(n, cap)
+                lo = max(p + 1 - window, 0) if window else 0
+                seen.append((b, np.arange(lo, max(hi, lo))))
+                rows.append(hi <= case.lengths[b])  # (tokens 48..52 of the first sequence hold anything)
+        keep = [t for t, ok in enumerate(rows) if ok]
+        check_seen(case, q[keep], out[keep], lse[keep], [seen[t] for t in keep])
