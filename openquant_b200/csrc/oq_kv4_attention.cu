@@ -29,6 +29,8 @@
 // (16: 88 us with one block a step, 86 us with two and spills; 20: 117 us).
 // Deeper rings (6 stages: 82.8 us) and scores computed a step ahead (85 us) cost
 // more than they hide.
+#include <climits>
+
 #include "oq_kv4_attention.cuh"
 
 namespace oq {
@@ -266,18 +268,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
         // blocks of this part; a sequence of length 0 has one without tokens
         const int nblk = first_tok < w.length ? i1 - i0 : 0;
 
-        // Row numbers / 16 in the cache of the next 32 blocks, one a lane.
+        // The page of block i of this part; negative: none that is in the cache.
+        const int pp = a.page_size >> 4;
+        auto page_of = [&](int i, int &blk) {
+            blk = w.b0 + i0 + i;
+            const int pg = blk / pp, page = __ldg(a.batch.table + (int64_t)b * a.batch.max_pages + pg);
+            blk -= pg * pp;
+            return page < a.pages ? page : -1;
+        };
+        // Row numbers / 16 in the cache of the next 32 blocks, one a lane.  Blocks
+        // without a page stand at row 0; where there are any (true), all_vis becomes
+        // INT_MIN: every step from then on is masked.
         uint32_t rows16 = 0;
         auto look_up = [&](int n0) {
             rows16 = 0;
+            bool none = false;
             if (n0 + lane < nblk) {
-                const int blk = w.b0 + i0 + n0 + lane, pp = a.page_size >> 4, pg = blk / pp;
-                const int page = __ldg(a.batch.table + (int64_t)b * a.batch.max_pages + pg);
-                if (page < 0 || page >= a.pages)
+                int blk;
+                const int page = page_of(n0 + lane, blk);
+                none = page < 0;
+                if (none)
                     index_error();
                 else
-                    rows16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * pp + (blk - pg * pp));
+                    rows16 = (uint32_t)(((int64_t)page * a.kv_heads + head) * pp + blk);
             }
+            return __any_sync(0xffffffffu, none) != 0;
         };
         auto load = [&](int i, int at) {  // block i, staged at byte `at` of the ring
             if (i < nblk) {
@@ -292,7 +307,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                 if (lane < 4 * NG) cp16(dst + 2 * kCodes + lane * 16, sc_lane + (size_t)r16 * kScales);
             }
         };
-        look_up(0);
+        const bool holes = look_up(0);
         __syncwarp();  // the ring's last reads (of the item before) are done
 #pragma unroll
         for (int i = 0; i < kStages; ++i) {
@@ -350,6 +365,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             const int last = min(row0 + kCols, w.rows) - 1;
             all_low = (int)max((int64_t)w.base + last / a.ratio + 1 - a.window, (int64_t)0);
         }
+        if (holes) all_vis = INT_MIN;
 
         float o[NT][HD / 16][4], m[NT][2], l[NT][2], most[NT][2];  // most: the score at which m is raised
 #pragma unroll
@@ -442,8 +458,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             // ---- weights p = 2^(s f - m)
             // some column misses some token of the blocks, or a block is not there
             const bool edge = tok + 16 * H > all_vis || tok < all_low || i + H > nblk;
+            bool lost[H] = {};  // block i + h is not there
             if (edge) {
                 const int64_t window = a.window > 0 ? a.window : INT32_MAX;
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    int blk;
+                    lost[h] = i + h >= nblk;
+                    if (all_vis == INT_MIN && !lost[h]) lost[h] = page_of(i + h, blk) < 0;
+                }
 #pragma unroll
                 for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -452,7 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                         for (int e = 0; e < 4; ++e) {
                             const int tk = tok + 16 * h + g + (e >> 1) * 8, p = pos[j][e & 1];
                             const int vis = a.causal ? p + 1 : w.length;
-                            if (tk >= vis || tk <= p - window || i + h >= nblk) s[h][j][e] = -INFINITY;
+                            if (tk >= vis || tk <= p - window || lost[h]) s[h][j][e] = -INFINITY;
                         }
             }
             bool raise = false;
@@ -526,7 +549,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const int tk = tok + 16 * h + 2 * t4 + (k & 1) + (k >> 1) * 8;
-                        if (tk >= w.length || tk < w.floor || i + h >= nblk) sc[k] = __ushort_as_half(0);
+                        if (tk >= w.length || tk < w.floor || lost[h]) sc[k] = __ushort_as_half(0);
                     }
                 }
                 const __half2 sa = __halves2half2(sc[0], sc[1]), sb = __halves2half2(sc[2], sc[3]);
@@ -554,7 +577,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             }
             __syncwarp();
             // later blocks take the place of these
-            if (((i + kStages) & 31) == 0) look_up(i + kStages);
+            if (((i + kStages) & 31) == 0 && look_up(i + kStages)) all_vis = INT_MIN;
 #pragma unroll
             for (int h = 0; h < H; ++h) load(i + kStages + h, at + h * kStage);
             cp_commit();

@@ -144,3 +144,67 @@ def test_attention_beyond_the_page_table(dim, heads, counts, window, causal):
                 rows.append(hi <= case.lengths[b])  # (tokens 48..52 of the first sequence hold anything)
         keep = [t for t, ok in enumerate(rows) if ok]
         check_seen(case, q[keep], out[keep], lse[keep], [seen[t] for t in keep])
+
+
+BAD_PAGES = [-1, 1 << 20, (1 << 31) - 1, -(1 << 31)]
+
+
+@pytest.mark.parametrize("dim, group, kv_heads, heads, lengths, counts, page, window, causal", [
+    (128, 32, 2, 8, [200, 37, 16, 1], [1, 1, 1, 1], 16, 0, True),       # single tokens
+    (64, 64, 2, 6, [500, 90], [5, 20], 32, 70, True),                   # a few rows, a window
+    (128, 128, 1, 8, [700, 90, 300], [130, 90, 1], 16, 0, True),        # prompts: the other kernel
+    (64, 32, 2, 4, [900, 200], [200, 150], 48, 0, False),
+    (128, 64, 1, 2, [5003], [40], 64, 0, True),                         # prompts over shared-out tokens
+    (64, 32, 1, 2, [4100], [64], 16, 3000, True),
+])
+def test_attention_leaves_out_pages_that_are_not_there(dim, group, kv_heads, heads, lengths, counts, page, window, causal):
+    """Tokens of a page number outside the cache are as if masked: page 0 does
+    not stand in for them."""
+    case = Case(lengths, counts, kv_heads, dim, group, page, seed=dim + heads, junk=True)
+    rng = np.random.default_rng(dim)
+    gone = [set() for _ in lengths]
+    table = case.table.copy()
+    for b, n in enumerate(lengths):
+        slots = -(-n // page)
+        for i in range(slots):
+            if rng.random() < 0.25 or i in (slots // 2,) or table[b, i] == 0:
+                table[b, i] = BAD_PAGES[rng.integers(4)]
+                gone[b].add(i)
+    case.batch.page_table.copy_(torch.from_numpy(table))
+    q = case.queries(heads, dim, torch.float16)
+    outs = []
+    for junk in (1.0, float("nan")):
+        case.cache.k_scales[0] = junk
+        case.cache.v_scales[0] = junk
+        outs.append(case.cache.attention(q, case.batch, window=window, causal=causal, return_log_sum=True))
+        assert device_error() == 3
+    seen = []
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        there = np.array([j // page not in gone[b] for j in range(n)])
+        for p in range(n - c, n):
+            hi = p + 1 if causal else n
+            lo = max(p + 1 - window, 0) if window else 0
+            idx = np.arange(lo, max(hi, lo))
+            seen.append((b, idx[there[idx]]))
+    check_seen(case, q, *outs[1], seen)
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+
+
+def test_attention_leaves_out_pages_of_long_shares():
+    """Forty sequences over the same pages, each without other ones of them:
+    a warp's share is more blocks than one look-up covers."""
+    from openquant_b200.kv_cache import KVBatch
+
+    case = Case([2560], [40], 16, 64, page=16, junk=True)
+    rng = np.random.default_rng(5)
+    table = np.repeat(case.table[:1], 40, 0)
+    there = rng.random(table.shape) > 0.02
+    there[3] = False
+    there[4] = True
+    table[~there] = -1
+    dev = dict(dtype=torch.int32, device="cuda")
+    batch = KVBatch(torch.from_numpy(table).cuda(), torch.full((40,), 2560, **dev))
+    q = case.queries(16, 64, torch.bfloat16)
+    out, lse = case.cache.attention(q, batch, return_log_sum=True)
+    assert device_error() == 3
+    check_seen(case, q, out, lse, [(0, np.flatnonzero(np.repeat(row, 16))) for row in there])
