@@ -444,7 +444,9 @@ typedef struct {
  * count .. lengths[b] - 1.  starts NULL: one token per sequence, token b for
  * sequence b.  Tokens from starts[sequences] on are padding (attention gives
  * 0 for them, append skips them).  max_tokens is an upper bound of the tokens
- * per sequence.  At most 2048 sequences.  All arrays int32, on the device.
+ * per sequence, for which attention plans its launches: a sequence with more is
+ * left out there (0, log-sum -inf, device error 3).  At most 2048 sequences.
+ * All arrays int32, on the device.
  * A page number outside the cache, a position outside the page table or the
  * rotary table is not followed: the access is left out and the device error
  * becomes 3 (oq_take_device_error). */

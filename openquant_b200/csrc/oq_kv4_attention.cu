@@ -70,6 +70,7 @@ struct Work {
     int length, base;  // cached tokens that can be read; position of the step's first token
     int floor;         // first cached token any row sees
     int b0, nb, blocks;
+    bool out;  // left out: no blocks, and its rows are cleared by the joining kernel
 };
 
 __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
@@ -79,7 +80,8 @@ __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
     w.length = length_of(a.batch, b, a.page_size, end);
     w.base = end - w.count;
     w.rows = w.count * a.ratio;
-    w.blocks = w.rows > a.few ? 0 : (w.rows + cols - 1) / cols;
+    w.out = w.count > a.max_tokens;
+    w.blocks = w.rows > a.few || w.out ? 0 : (w.rows + cols - 1) / cols;
     w.floor = a.window > 0 ? (int)max((int64_t)w.base + 1 - a.window, (int64_t)0) : 0;
     w.b0 = w.floor >> 4;
     w.nb = max(((w.length + 15) >> 4) - w.b0, 1);
@@ -651,6 +653,18 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
     const bool late = quotient(c0 * all, shares) >= s;
     // (also by a CTA that has nothing to do: this kernel is not complete before the other)
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (w.out) {
+        // (here, as the streaming kernel's code begins cold at every launch: clearing
+        // them there cost one request of 1000 tokens 0.3 us of 10.75)
+        index_error();
+        const int64_t row0 = (int64_t)w.first * a.q_heads, row1 = row0 + (int64_t)w.count * a.q_heads;
+        int64_t row = row0 + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 8 + warp;
+        for (; row < row1; row += (int64_t)gridDim.x * gridDim.y * 8) {
+            for (int i = lane; i < HD; i += 32) put(static_cast<T *>(a.out) + row * HD + i, 0.0f);
+            if (lane == 0 && a.log_sum != nullptr) a.log_sum[row] = -INFINITY;
+        }
+        return;
+    }
     if (!there || c0 == c1) return;
     const int head = item / w.blocks, row0 = (item - head * w.blocks) * kCols;
     const float *first = a.parts + (c0 * 2 + (late ? 0 : 1)) * S::kPart;
@@ -884,6 +898,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     a.out = out;
     a.log_sum = log_sum;
     a.tokens = tokens;
+    a.max_tokens = batch->max_tokens;
     a.q_heads = q_heads;
     a.ratio = q_heads / cache->kv_heads;
     a.f = scale * 1.4426950408889634f;

@@ -24,10 +24,11 @@ struct AttnArgs {
     float f;             // scale * log2 e
     int64_t window;
     int causal;
-    float *parts;  // partial results
-    int vec;       // q rows 16-byte aligned
-    int few;       // sequences of at most `few` query rows a key head go to the streaming kernel,
-                   // the others to the prompt kernel
+    float *parts;    // partial results
+    int vec;         // q rows 16-byte aligned
+    int max_tokens;  // what the launches are planned for: a sequence with more tokens is left out
+    int few;         // sequences of at most `few` query rows a key head go to the streaming kernel,
+                     // the others to the prompt kernel
 };
 
 __device__ __forceinline__ float ex2(float x) {

@@ -145,7 +145,8 @@ __device__ __forceinline__ void st16(uint32_t addr, uint32_t a, uint32_t b, uint
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// What item `id` (over all sequences with more than a.few rows) works on.
+// What item `id` (over all sequences with more than a.few rows that are not
+// left out: the streaming work's joining kernel clears their rows) works on.
 struct Item {
     int b, first, count, rows, head, row0;
     int length, base;   // cached tokens that can be read; position of the step's first token
@@ -169,7 +170,7 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int id, int cuts, I
             int first, count;
             tokens_of(a.batch, b, a.tokens, first, count);
             const int64_t rows = (int64_t)count * a.ratio;
-            if (rows > a.few) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
+            if (rows > a.few && count <= a.max_tokens) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
         }
         int inc = n;
 #pragma unroll

@@ -222,7 +222,8 @@ class KVBatch:
     (starts[0] = 0): sequence b's tokens of the step's arrays are
     [starts[b], starts[b + 1]); None: one token per sequence.  Tokens from
     starts[-1] on are padding.  max_tokens: an upper bound of the tokens per
-    sequence, known on the host (needed with starts).
+    sequence, known on the host (needed with starts); attention leaves out a
+    sequence with more (rows of 0, log-sum -inf, device error 3).
 
     The tensors are read by the kernels, so their contents may change between
     steps (a captured CUDA graph replays with the new ones).  A page number or

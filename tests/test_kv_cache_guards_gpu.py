@@ -208,3 +208,26 @@ def test_attention_leaves_out_pages_of_long_shares():
     out, lse = case.cache.attention(q, batch, return_log_sum=True)
     assert device_error() == 3
     check_seen(case, q, out, lse, [(0, np.flatnonzero(np.repeat(row, 16))) for row in there])
+
+
+@pytest.mark.parametrize("dim, kv_heads, heads, lengths, counts, most", [
+    (128, 2, 16, [60, 90, 33], [5, 3, 4], 4),        # the longest would go to the other kernel, which is not launched
+    (128, 2, 8, [700, 1, 40], [4, 1, 1], 1),         # more blocks of rows than are joined
+    (64, 1, 2, [400, 300, 9], [300, 100, 9], 100),   # prompts
+    (64, 1, 4, [2000, 2100, 50], [1, 2000, 1], 64),
+])
+def test_attention_of_more_tokens_than_max_tokens(dim, kv_heads, heads, lengths, counts, most):
+    """A sequence with more of the step's tokens than the host was told is left
+    out, with an error; the others are whole."""
+    from openquant_b200.kv_cache import KVBatch
+
+    case = Case(lengths, counts, kv_heads, dim, page=16, seed=most, junk=True)
+    batch = KVBatch(case.batch.page_table, case.batch.lengths, case.batch.starts, max_tokens=most)
+    q = case.queries(heads, dim, torch.bfloat16)
+    out = torch.full_like(q, float("nan"))
+    _, lse = case.cache.attention(q, batch, out=out, return_log_sum=True)
+    assert device_error() == 3
+    seen = []
+    for b, (n, c) in enumerate(zip(lengths, counts)):
+        seen += [(b, np.arange(p + 1 if c <= most else 0)) for p in range(n - c, n)]
+    check_seen(case, q, out, lse, seen)
