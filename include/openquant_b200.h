@@ -443,7 +443,9 @@ typedef struct {
  * [starts[b], starts[b + 1]) of the step's arrays, at positions lengths[b] -
  * count .. lengths[b] - 1.  starts NULL: one token per sequence, token b for
  * sequence b.  Tokens from starts[sequences] on are padding (attention gives
- * 0 for them, append skips them).  max_tokens is an upper bound of the tokens
+ * 0 for them, append skips them).  A sequence whose starts are not in order
+ * within the arrays (starts[0] = 0) is left out: append skips its tokens, read
+ * and attention give 0, the device error becomes 3.  max_tokens is an upper bound of the tokens
  * per sequence, for which attention plans its launches: a sequence with more is
  * left out there (0, log-sum -inf, device error 3).  At most 2048 sequences.
  * All arrays int32, on the device.

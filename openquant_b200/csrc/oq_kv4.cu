@@ -287,13 +287,16 @@ rotary_kernel(Rows x, T *y, int64_t y_ts, int64_t y_hs, int64_t tokens, int head
 }
 
 // Place of the step's token t in its sequence, and its row of head 0 in the
-// cache (-1: none).  Returns false for a padding token.
+// cache (-1: none).  Returns false for a padding token, and with an error for
+// one of a sequence whose starts are not in order.
 __device__ __forceinline__ bool find_row(const Batch &bt, int seq, int64_t t, int64_t tokens, int64_t pages,
                                          int page_size, int kv_heads, int64_t &pos, int64_t &at) {
     if (seq >= bt.sequences) return false;
     int first, count;
-    tokens_of(bt, seq, tokens, first, count);
-    if (t < first || t >= first + count) return false;
+    if (!tokens_of(bt, seq, tokens, first, count) || t < first || t >= first + count) {
+        if ((threadIdx.x & 31) == 0) index_error();
+        return false;
+    }
     // The place that the length gives, inside the page-table row or not: a
     // length cut to the row would move the tokens onto others that are there.
     pos = (int64_t)__ldg(bt.lengths + seq) - count + (t - first);

@@ -43,18 +43,18 @@ struct Batch {
     int sequences, max_pages;
 };
 
-// starts[b] and the token count of sequence b, kept inside the step's array.
-__device__ __forceinline__ void tokens_of(const Batch &bt, int b, int64_t tokens, int &first, int &count) {
+// First token and token count of sequence b, kept inside the step's array.
+// False: its starts are not in order within the array (the first one at 0).
+__device__ __forceinline__ bool tokens_of(const Batch &bt, int b, int64_t tokens, int &first, int &count) {
     if (bt.starts == nullptr) {
         first = b;
         count = b < tokens ? 1 : 0;
-        return;
+        return true;
     }
-    int s = __ldg(bt.starts + b), e = __ldg(bt.starts + b + 1);
-    s = min(max(s, 0), (int)tokens);
-    e = min(max(e, s), (int)tokens);
-    first = s;
-    count = e - s;
+    const int s = __ldg(bt.starts + b), e = __ldg(bt.starts + b + 1);
+    first = b == 0 ? 0 : min(max(s, 0), (int)tokens);
+    count = min(max(e, first), (int)tokens) - first;
+    return s == first && e == first + count;
 }
 
 // Cached tokens of sequence b that its page-table row has room for; `end`: its

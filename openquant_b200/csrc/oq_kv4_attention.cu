@@ -75,12 +75,11 @@ struct Work {
 
 __device__ __forceinline__ Work work_of(const Args &a, int b, int cols) {
     Work w;
-    tokens_of(a.batch, b, a.tokens, w.first, w.count);
+    w.out = !tokens_of(a.batch, b, a.tokens, w.first, w.count) || w.count > a.max_tokens;
     int end;
     w.length = length_of(a.batch, b, a.page_size, end);
     w.base = end - w.count;
     w.rows = w.count * a.ratio;
-    w.out = w.count > a.max_tokens;
     w.blocks = w.rows > a.few || w.out ? 0 : (w.rows + cols - 1) / cols;
     w.floor = a.window > 0 ? (int)max((int64_t)w.base + 1 - a.window, (int64_t)0) : 0;
     w.b0 = w.floor >> 4;

@@ -168,9 +168,9 @@ __device__ __forceinline__ bool find_item(const AttnArgs &a, int id, int cuts, I
         int n = 0;
         if (b < a.batch.sequences) {
             int first, count;
-            tokens_of(a.batch, b, a.tokens, first, count);
+            const bool ok = tokens_of(a.batch, b, a.tokens, first, count);
             const int64_t rows = (int64_t)count * a.ratio;
-            if (rows > a.few && count <= a.max_tokens) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
+            if (rows > a.few && ok && count <= a.max_tokens) n = (int)((rows + kPromptRows - 1) / kPromptRows) * a.kv_heads;
         }
         int inc = n;
 #pragma unroll

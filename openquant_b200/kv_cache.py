@@ -227,8 +227,9 @@ class KVBatch:
 
     The tensors are read by the kernels, so their contents may change between
     steps (a captured CUDA graph replays with the new ones).  A page number or
-    position outside its array is not followed: the device error
-    (oq_take_device_error) becomes 3.
+    position outside its array is not followed, and a sequence whose starts
+    are not in order within the step's arrays is left out (nothing is written,
+    rows of 0): the device error (oq_take_device_error) becomes 3.
     """
 
     def __init__(self, page_table, lengths, starts=None, *, max_tokens=None):

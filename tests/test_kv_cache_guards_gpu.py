@@ -231,3 +231,73 @@ def test_attention_of_more_tokens_than_max_tokens(dim, kv_heads, heads, lengths,
     for b, (n, c) in enumerate(zip(lengths, counts)):
         seen += [(b, np.arange(p + 1 if c <= most else 0)) for p in range(n - c, n)]
     check_seen(case, q, out, lse, seen)
+
+
+@pytest.mark.parametrize("starts, tokens, whole", [
+    ([0, 5], 4, []),                 # fewer tokens in the step's arrays than starts says
+    ([2, 4], 4, []),                 # the first sequence does not begin at 0
+    ([0, -1, 4], 4, []),
+    ([0, 2, (1 << 31) - 1], 40, [0]),
+    ([-(1 << 31), 3, 6], 6, [1]),
+])
+@pytest.mark.parametrize("heads", [2, 16])
+def test_starts_that_are_not_in_order(starts, tokens, whole, heads):
+    """Such a sequence is left out, with an error: nothing is written for it,
+    its rows are 0.  Sequences apart from it are whole."""
+    from openquant_b200.kv_cache import Int4KVCache, KVBatch
+
+    dev = dict(dtype=torch.int32, device="cuda")
+    n = len(starts) - 1
+    cache = Int4KVCache.allocate(4 * n, 16, 1, 64)
+    pages = torch.arange(4 * n, **dev).view(n, 4)
+    fill = torch.randn(64 * n, 1, 64, device="cuda").half()
+    cache.append(fill, fill, KVBatch(pages, torch.full((n,), 64, **dev),
+                                     torch.arange(n + 1, **dev) * 64, max_tokens=64))
+    assert device_error() == 0
+    before = [x.clone() for x in (cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales)]
+    lengths = torch.full((n,), 50, **dev)
+    batch = KVBatch(pages, lengths, torch.tensor(starts, **dev), max_tokens=40)
+    k, q = torch.randn(tokens, 1, 64, device="cuda").half(), torch.randn(tokens, heads, 64, device="cuda").half()
+    cache.append(k, k, batch)
+    assert device_error() == 3
+    own = {b: range(starts[b], starts[b + 1]) for b in whole}
+    rows = torch.zeros(4 * n, 16, dtype=torch.bool, device="cuda")
+    for b, r in own.items():
+        for i in range(len(r)):
+            j = 50 - len(r) + i
+            rows[4 * b + j // 16, j % 16] = True
+    for x, y in zip((cache.k_codes, cache.k_scales, cache.v_codes, cache.v_scales), before):
+        assert torch.equal(x[~rows[:, None].expand(-1, 1, -1)], y[~rows[:, None].expand(-1, 1, -1)])
+    got = cache.read(batch, tokens)[0]
+    assert device_error() == 3
+    out = torch.full_like(q, float("nan"))
+    cache.attention(q, batch, out=out)
+    assert device_error() == 3
+    for b, r in own.items():
+        one = KVBatch(pages[b:b + 1].contiguous(), lengths[:1], torch.tensor([0, len(r)], **dev), max_tokens=40)
+        s = slice(r.start, r.stop)
+        assert torch.equal(got[s], cache.read(one, len(r))[0])
+        assert (out[s] - cache.attention(q[s], one)).abs().max() <= 2 * (2.0**-11 * 5 + 2.0**-9 * 5)
+    left = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    for r in own.values():
+        left[r.start:r.stop] = False
+    assert not got[left].any()
+    assert not out[left].any()
+    assert device_error() == 0
+
+
+@pytest.mark.parametrize("starts", [[0, 3, 2, 5], [0, 5, 1, 2, 9], [0, 9, 0, 9]])
+def test_starts_of_sequences_that_overlap(starts):
+    """Nothing says whose a token is: an error."""
+    from openquant_b200.kv_cache import Int4KVCache, KVBatch
+
+    dev = dict(dtype=torch.int32, device="cuda")
+    n, tokens = len(starts) - 1, starts[-1]
+    cache = Int4KVCache.allocate(n, 64, 1, 64)
+    batch = KVBatch(torch.arange(n, **dev).view(n, 1), torch.full((n,), 50, **dev), torch.tensor(starts, **dev),
+                    max_tokens=40)
+    k = torch.randn(tokens, 1, 64, device="cuda").half()
+    for call in (lambda: cache.append(k, k, batch), lambda: cache.read(batch, tokens),
+                 lambda: cache.attention(k, batch)):
+        call()
+        assert device_error() == 3
