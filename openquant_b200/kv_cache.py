@@ -20,7 +20,8 @@ A step of a serving loop, for each layer:
     y = cache.attention(q, batch)
 
 Everything is asynchronous on the current CUDA stream of the tensors' GPU.
-There is no CPU fallback.
+Only rotary() has a gradient: the cache is for inference, and what append, read
+and attention return carries no history.  There is no CPU fallback.
 """
 from __future__ import annotations
 
@@ -167,6 +168,21 @@ def _call(dev, fn, *args):
         nat.check(st)
 
 
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, table, positions, interleaved, inverse):
+        ctx.save_for_backward(table, positions)
+        ctx.interleaved, ctx.inverse = interleaved, inverse
+        return rotary(x, table, positions, interleaved=interleaved, inverse=inverse)
+
+    @staticmethod
+    def backward(ctx, g):
+        table, positions = ctx.saved_tensors
+        if g.stride(2) != 1:
+            g = g.contiguous()
+        return rotary(g, table, positions, interleaved=ctx.interleaved, inverse=not ctx.inverse), None, None, None, None
+
+
 def rotary(x, table, positions, *, interleaved=False, inverse=False, out=None):
     """Rotary positions: x [tokens, heads, head_dim] (fp32, fp16 or bf16 on a
     GPU; tokens and heads may be strided) with every token's heads turned by
@@ -175,8 +191,12 @@ def rotary(x, table, positions, *, interleaved=False, inverse=False, out=None):
     table (rotary_table) has one row per position; its width, the rotary
     dimension, may be less than head_dim (the rest of a head is copied).
     Pairs are (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved=True:
-    (a, b) becomes (a cos - b sin, b cos + a sin).  inverse=True turns back --
-    the gradient of the rotation with respect to x.  out may be x itself.
+    (a, b) becomes (a cos - b sin, b cos + a sin).  inverse=True turns by the
+    negative angle: the transpose of the rotation, which takes the gradient of
+    y to that of x (and y back to x, where the table's magnitude is 1).  out may
+    be x itself.  Where x needs a gradient the call is recorded by autograd,
+    its gradient being the same kernel with the other sign; out cannot be given
+    then, and the table has no gradient.
     positions (int32 or int64 [tokens]) outside the table leave their tokens'
     output unwritten and set the device error (oq_take_device_error) to 3.
     """
@@ -187,6 +207,12 @@ def rotary(x, table, positions, *, interleaved=False, inverse=False, out=None):
     spec = _rotary_spec(table, (_ROTARY_INTERLEAVED if interleaved else 0) | (_ROTARY_INVERSE if inverse else 0), dim,
                         dev)
     pos, wide = _positions(positions, tokens, dev)
+    if (x.requires_grad or table.requires_grad) and torch.is_grad_enabled():
+        if table.requires_grad:
+            raise ValueError("the table has no gradient")
+        if out is not None:
+            raise ValueError("out cannot be given where x needs a gradient")
+        return _Rotary.apply(x, table, positions, bool(interleaved), bool(inverse))
     if out is None:
         out = _like(x)
     elif (out.shape != x.shape or out.dtype is not x.dtype or out.get_device() != dev

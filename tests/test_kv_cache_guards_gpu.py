@@ -301,3 +301,42 @@ def test_starts_of_sequences_that_overlap(starts):
                  lambda: cache.attention(k, batch)):
         call()
         assert device_error() == 3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rotary_is_recorded_by_autograd(dtype, interleaved, inverse):
+    from openquant_b200.kv_cache import rotary, rotary_table
+
+    kw = dict(interleaved=interleaved, inverse=inverse)
+    table, pos = rotary_table(300, 48, scaling={"type": "parts", "factor": 4.0, "original_positions": 256}), \
+        torch.arange(9, device="cuda") * 31
+    wide = torch.randn(9, 5 * 64, device="cuda").to(dtype).requires_grad_()
+    x = wide.unflatten(1, (5, 64))[:, 1:4]  # strided heads
+    y = rotary(x, table, pos, **kw)
+    assert y.requires_grad and torch.equal(y.detach(), rotary(x.detach(), table, pos, **kw))
+    g = torch.randn(9, 3, 64, device="cuda").to(dtype)
+    (got,) = torch.autograd.grad(y, wide, g, retain_graph=True)
+    # the formula's: the transpose, a pair (a, b) of g to (a cos + b sin, b cos - a sin)
+    want = ko.rotate(f64(g).astype(np.float32), table.cpu().numpy(), pos.cpu().numpy(), interleaved, not inverse)
+    got = got.unflatten(1, (5, 64))
+    assert torch.equal(got[:, 1:4].cpu(), torch.from_numpy(want).to(dtype))
+    assert not got[:, 0].any() and not got[:, 4].any()
+    # a gradient that is one number everywhere (no stride), as sum() gives
+    (ones,) = torch.autograd.grad(y.sum(), wide)
+    full = ko.rotate(np.ones((9, 3, 64), np.float32), table.cpu().numpy(), pos.cpu().numpy(), interleaved, not inverse)
+    assert torch.equal(ones.unflatten(1, (5, 64))[:, 1:4].cpu(), torch.from_numpy(full).to(dtype))
+    if dtype is torch.float32:  # differences along a direction: the rotation is linear
+        d = torch.randn(9, 3, 64, device="cuda")
+        diff = (rotary(x.detach() + d, table, pos, **kw).double() - rotary(x.detach() - d, table, pos, **kw).double()) / 2
+        lhs, rhs = (diff * g.double()).sum(), (d.double() * got[:, 1:4].double()).sum()
+        # 1728 terms of about 1, each with a few fp32 roundings of values up to ~8
+        assert abs(float(lhs - rhs)) <= 1728 * 8 * 8 * 2.0**-24
+    with torch.no_grad():
+        assert not rotary(x, table, pos, **kw).requires_grad
+    with pytest.raises(ValueError, match="out"):
+        rotary(x, table, pos, out=torch.empty_like(g), **kw)
+    with pytest.raises(ValueError, match="gradient"):
+        rotary(x, table.clone().requires_grad_(), pos, **kw)
+    assert device_error() == 0
