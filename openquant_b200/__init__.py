@@ -9,7 +9,7 @@ include/openquant_b200.h) behind the reference package's Python API:
   openquant_b200.gpu_benchmark  decode_gpu
   openquant_b200.group_benchmark restore_groupwise_torch
   openquant_b200.triton_int4    int4_linear
-  openquant_b200.kv_cache       Int4KVCache, KVBatch, rotary, rotary_table
+  openquant_b200.kv_cache       Int4KVCache, KVBatch, rotary, rotary_table, take_device_error
   openquant_b200.cli            main (`openquant gpu|tune|cpu|report`)
 
 The top-level `openquant` package re-exports these under the reference's

@@ -34,13 +34,25 @@ import torch
 from . import _native as nat
 from .triton_int4 import _stream_handle
 
-__all__ = ["rotary_table", "rotary", "KVBatch", "Int4KVCache"]
+__all__ = ["rotary_table", "rotary", "KVBatch", "Int4KVCache", "take_device_error"]
 
 _CODES = {torch.float32: nat.OQ_F32, torch.float16: nat.OQ_F16, torch.bfloat16: nat.OQ_BF16}
 _ROTARY_INTERLEAVED, _ROTARY_INVERSE = 1, 2
 _NOT_CAUSAL = 1
 MAX_SEQUENCES = 2048
 _KEEP_BYTES, _KEEP_BUFFERS = 32 << 20, 4  # workspaces that a KVBatch keeps
+
+
+def take_device_error():
+    """Reads and clears the library's device error word of the current GPU,
+    after the work on it has ended: 0, or what a kernel met first -- 1 gave up
+    waiting inside a kernel (its outputs are undefined), 2 for a peer GPU, 3 a
+    page number, position or start of a sequence outside its array (the access
+    was left out)."""
+    nat.require_device()
+    code = ctypes.c_int32()
+    nat.check(nat.load().oq_take_device_error(ctypes.byref(code)))
+    return code.value
 
 
 # -------------------------------------------------------------- rotary --
@@ -198,7 +210,7 @@ def rotary(x, table, positions, *, interleaved=False, inverse=False, out=None):
     its gradient being the same kernel with the other sign; out cannot be given
     then, and the table has no gradient.
     positions (int32 or int64 [tokens]) outside the table leave their tokens'
-    output unwritten and set the device error (oq_take_device_error) to 3.
+    output unwritten and set the device error (take_device_error) to 3.
     """
     tokens, heads, dim = _heads(x, "x", (torch.float32, torch.float16, torch.bfloat16))
     if dim % 8 or dim > 256:
@@ -255,7 +267,7 @@ class KVBatch:
     steps (a captured CUDA graph replays with the new ones).  A page number or
     position outside its array is not followed, and a sequence whose starts
     are not in order within the step's arrays is left out (nothing is written,
-    rows of 0): the device error (oq_take_device_error) becomes 3.
+    rows of 0): the device error (take_device_error) becomes 3.
     """
 
     def __init__(self, page_table, lengths, starts=None, *, max_tokens=None):

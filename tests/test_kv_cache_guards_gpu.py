@@ -340,3 +340,13 @@ def test_rotary_is_recorded_by_autograd(dtype, interleaved, inverse):
     with pytest.raises(ValueError, match="gradient"):
         rotary(x, table.clone().requires_grad_(), pos, **kw)
     assert device_error() == 0
+
+
+def test_take_device_error():
+    from openquant_b200.kv_cache import rotary, rotary_table, take_device_error
+
+    assert take_device_error() == 0
+    x, table = torch.randn(1, 2, 64, device="cuda"), rotary_table(10, 64)
+    rotary(x, table, torch.tensor([10], device="cuda"))
+    rotary(x, table, torch.tensor([9], device="cuda"))
+    assert take_device_error() == 3 and take_device_error() == 0
