@@ -770,6 +770,13 @@ int columns_of(const oq_kv4_cache *c, const oq_kv4_batch *b, int q_heads) {
     return (int64_t)b->max_tokens * (q_heads / c->kv_heads) <= 8 ? 1 : 2;
 }
 
+// Items of a sequence that the streaming kernel may have to join: a block of
+// the joining kernel's grid in y.
+int64_t join_items(int kv_heads, int ratio, int few, const oq_kv4_batch *b, int nt) {
+    const int64_t most = (int64_t)b->max_tokens * ratio;
+    return cdiv(most < few ? most : few, 8 * nt) * kv_heads;
+}
+
 template <typename T, int HD, int GS, int NT>
 int stream_launch(Args &a, const oq_kv4_batch *batch, bool beside, cudaStream_t st) {
     const int share = share_of<HD, NT>();
@@ -792,9 +799,7 @@ int stream_launch(Args &a, const oq_kv4_batch *batch, bool beside, cudaStream_t 
         return OQ_ERR_CUDA;
     }
 
-    const int64_t most = (int64_t)batch->max_tokens * a.ratio;
-    const int64_t blocks = cdiv(most < a.few ? most : a.few, 8 * NT), items = blocks * a.kv_heads;
-    OQ_REQUIRE(items <= 65535, "kv4_attention: too many key heads");
+    const int64_t items = join_items(a.kv_heads, a.ratio, a.few, batch, NT);
     const int warps = share * kWarps;
     const bool split = warps > 16 * items * batch->sequences;
     cfg.gridDim = dim3(split ? Shape<HD, NT>::kSlices : 1, (unsigned)items, batch->sequences);
@@ -909,6 +914,8 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     const int64_t most = (int64_t)batch->max_tokens * a.ratio;  // rows a sequence and key head
     a.few = few_rows(cache, q_heads);
+    // (before any launch: a refused call does nothing)
+    OQ_REQUIRE(join_items(a.kv_heads, a.ratio, a.few, batch, nt) <= 65535, "kv4_attention: too many key heads");
     const bool beside = most > a.few;
     if (beside) {
         AttnArgs p = a;

@@ -71,3 +71,18 @@ def test_rotary_scaling_by_parts_is_a_line_between_the_turning_points(dim, base,
             assert got[i] == plain[i]
         if t <= base ** (-2 / dim):
             assert math.isclose(float(got[i]), float(plain[i]) / factor, rel_tol=1e-12)
+
+
+def test_too_many_key_heads_are_refused_before_anything_is_launched():
+    import ctypes
+
+    from openquant_b200 import _native as nat, build, kv_cache as kc
+
+    build.build()
+    lib, p = nat.load(), 1 << 20
+    cache = kc._Cache(p, p, p, p, 4, 16, 40000, 128, 32)
+    batch = kc._Batch(p, p, None, 2, 2, 1)
+    heads = 32 * 40000  # two blocks of 16 rows a key head: 80000 items
+    st = lib.oq_kv4_attention(ctypes.byref(cache), ctypes.byref(batch), p, nat.OQ_F16, heads, heads * 128, 128, p, None,
+                              2, 1.0, 0, 0, p, 1 << 40, None)
+    assert st == nat.OQ_ERR_INVALID and "key heads" in nat.last_error()
