@@ -299,6 +299,8 @@ class KVBatch:
         max_tokens = int(max_tokens)
         if max_tokens < 1 or (starts is None and max_tokens != 1):
             raise ValueError("max_tokens must be positive, and 1 without starts")
+        if max_tokens >= 1 << 31:
+            raise ValueError("max_tokens must be below 2^31")
         self.page_table, self.lengths, self.starts = page_table, lengths, starts
         self.sequences, self.max_tokens = n, max_tokens
         self._dev = dev

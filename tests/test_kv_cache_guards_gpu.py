@@ -350,3 +350,14 @@ def test_take_device_error():
     rotary(x, table, torch.tensor([10], device="cuda"))
     rotary(x, table, torch.tensor([9], device="cuda"))
     assert take_device_error() == 3 and take_device_error() == 0
+
+
+def test_max_tokens_beyond_32_bits_is_refused():
+    from openquant_b200.kv_cache import KVBatch
+
+    dev = dict(dtype=torch.int32, device="cuda")
+    args = torch.zeros(1, 1, **dev), torch.ones(1, **dev), torch.tensor([0, 5], **dev)
+    assert KVBatch(*args, max_tokens=(1 << 31) - 1).max_tokens == (1 << 31) - 1
+    for n in (1 << 31, (1 << 32) + 1):  # (the second would be 1 in 32 bits)
+        with pytest.raises(ValueError, match="2\\^31"):
+            KVBatch(*args, max_tokens=n)
