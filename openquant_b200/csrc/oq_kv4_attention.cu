@@ -906,7 +906,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     a.q_heads = q_heads;
     a.ratio = q_heads / cache->kv_heads;
     a.f = scale * 1.4426950408889634f;
-    a.window = window;
+    a.window = window < INT32_MAX ? window : 0;  // positions are below 2^31: no limit
     a.causal = (flags & OQ_KV4_NOT_CAUSAL) ? 0 : 1;
     a.parts = static_cast<float *>(workspace);
     a.vec = aligned(q, 16) && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;

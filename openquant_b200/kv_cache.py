@@ -492,6 +492,7 @@ class Int4KVCache:
         window = int(window or 0)
         if window < 0:
             raise ValueError("window must not be negative")
+        window = min(window, 1 << 31)  # no limit
         scale = dim ** -0.5 if scale is None else float(scale)
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")

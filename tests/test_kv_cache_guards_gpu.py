@@ -361,3 +361,20 @@ def test_max_tokens_beyond_32_bits_is_refused():
     for n in (1 << 31, (1 << 32) + 1):  # (the second would be 1 in 32 bits)
         with pytest.raises(ValueError, match="2\\^31"):
             KVBatch(*args, max_tokens=n)
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 2, (1 << 31) - 1, 1 << 31, (1 << 63) - 1, (1 << 64) + 5])
+@pytest.mark.parametrize("causal", [False, True])
+def test_attention_windows_without_end(window, causal):
+    """As without a window, for tokens before a sequence's start too."""
+    case = Case([3, 200, 90], [3, 1, 70], 2, 64, junk=True)
+    case.batch.lengths[0] = 2  # its first token is at position -1
+    q = case.queries(4, 64, torch.float16)
+    out, lse = case.cache.attention(q, case.batch, causal=causal, return_log_sum=True)
+    got = case.cache.attention(q, case.batch, window=window, causal=causal, return_log_sum=True)
+    assert torch.equal(got[0], out) and torch.equal(got[1], lse)
+    seen = []
+    for b, (n, c) in enumerate(zip([2, 200, 90], case.counts)):
+        seen += [(b, np.arange(max(p + 1, 0) if causal else n)) for p in range(n - c, n)]
+    check_seen(case, q, *got, seen)
+    assert device_error() == 0
