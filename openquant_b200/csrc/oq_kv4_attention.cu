@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             l[j][0] = l[j][1] = 0.0f;
         }
 
-        int at = 0;  // byte of the step in the ring
+        bool huge = false;  // a maximum of this lane's columns passed kHuge
+        int at = 0;         // byte of the step in the ring
         for (int i = 0; i < nblk; i += H) {
             cp_wait<kSteps - 1>();
             __syncwarp();
@@ -487,6 +488,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
 #pragma unroll
                     for (int e = 0; e < 4; ++e) raise |= s[h][j][e] > most[j][e & 1];
             if (__any_sync(0xffffffffu, raise)) {
+                huge = false;
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -496,10 +498,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
                         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-                        const float mn = fmaxf(m[j][e], mx * f[j][e] - kLift);
+                        const float mn = fmaxf(m[j][e], __fmul_rn(mx, f[j][e]) - kLift);
                         const float corr = ex2(m[j][e] - mn);
                         m[j][e] = mn;
-                        most[j][e] = mn > -1e30f ? __fdividef(mn + kRaise, f[j][e]) : -INFINITY;
+                        // (-1e30, nothing seen yet, passes kHuge too)
+                        most[j][e] = fabsf(mn) > kHuge ? -INFINITY : __fdividef(mn + kRaise, f[j][e]);
+                        huge |= fabsf(mn) > kHuge;
                         l[j][e] *= corr;
 #pragma unroll
                         for (int i2 = 0; i2 < HD / 16; ++i2) {
@@ -507,6 +511,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                             o[j][i2][e + 2] *= corr;
                         }
                     }
+                if (huge) {
+                    // (a column's lanes agree; from now on every step comes here)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        most[j][0] = most[j][1] = -INFINITY;
+#pragma unroll
+                        for (int h = 0; h < H; ++h)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[h][j][e] = __fmul_rn(s[h][j][e], f[j][e & 1]);
+                    }
+                }
             }
             uint32_t pf[H][NT][2];
 #pragma unroll
@@ -516,7 +531,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                     float p[4];
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[e] = ex2(fmaf(s[h][j][e], f[j][e & 1], -m[j][e & 1]));
+                        p[e] = ex2(fmaf(s[h][j][e], huge ? 1.0f : f[j][e & 1], -m[j][e & 1]));
                         l[j][e & 1] += p[e];
                     }
                     pf[h][j][0] = transpose8x8(as_u32(__floats2half2_rn(p[0], p[1])));

@@ -9,6 +9,11 @@ namespace kv4 {
 constexpr float kLift = 6.0f;    // a running maximum is set this much below the largest score (log2)
 constexpr float kRaise = 14.0f;  // and raised when a score passes it by more than this
 
+// Scores beyond this (log2) are rounded to fp32 before the maximum is taken off.
+// One fused operation would take the exact product s f less a maximum that was
+// rounded: up to |s f| 2^-23 too much, and from 2^24 on p may pass fp16.
+constexpr float kHuge = 1048576.0f;
+
 struct AttnArgs {
     const uint8_t *k_codes, *v_codes;
     const __half *k_scales, *v_scales;

@@ -352,6 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + quarter + kS + wg * kTok, to = tmem + quarter + kO + wg * HD;
             float m = -1e30f;
+            float lim = -INFINITY, fe = f;  // m is raised above it; what s is multiplied with in p
             float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             bool ok = __all_sync(0xffffffffu, wait(scanned, 0));
             const bool holes = *holes_at != 0;
@@ -388,10 +389,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                         mx[i] = fmaxf(fmaxf(mx[i], __uint_as_float(s[i][e])), __uint_as_float(s[i][e + 1]));
                     mx[i] = fmaxf(mx[i], __uint_as_float(s[i][31]));
                 }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * f;
-                const bool raise = top > m + kRaise;
-                if (__any_sync(0xffffffffu, raise)) {
-                    const float mn = raise ? top - kLift : m, corr = ex2(m - mn);
+                const float top = __fmul_rn(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])), f);
+                if (__any_sync(0xffffffffu, top > lim)) {
+                    const float mn = top - m > kRaise ? top - kLift : m, corr = ex2(m - mn);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) l2[i].x *= corr, l2[i].y *= corr;
                     m = mn;
@@ -406,8 +406,22 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             tmem_st_32x32b_x8(to + 8 * i, o);
                         }
                     }
+                    // (a row that has passed kHuge comes here with every block)
+                    const bool huge = m > -1e30f && fabsf(m) > kHuge;
+                    lim = m > -1e30f && !huge ? m + kRaise : -INFINITY;
+                    fe = huge ? 1.0f : f;
+                    if (huge) {
+#pragma unroll
+                        for (int i = 0; i < kTok; i += 2) {
+                            const float2 x = __fmul2_rn(make_float2(__uint_as_float(s[i >> 5][i & 31]),
+                                                                    __uint_as_float(s[i >> 5][(i & 31) + 1])),
+                                                        make_float2(f, f));
+                            s[i >> 5][i & 31] = __float_as_uint(x.x);
+                            s[i >> 5][(i & 31) + 1] = __float_as_uint(x.y);
+                        }
+                    }
                 }
-                const float2 f2 = make_float2(f, f), m2 = make_float2(-m, -m);
+                const float2 f2 = make_float2(fe, fe), m2 = make_float2(-m, -m);
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
                     uint32_t p[16];

@@ -378,3 +378,56 @@ def test_attention_windows_without_end(window, causal):
         seen += [(b, np.arange(max(p + 1, 0) if causal else n)) for p in range(n - c, n)]
     check_seen(case, q, *got, seen)
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("count", [1, 200])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("scale", [1e4, -1e6, 1e7, 1e8, 1e10, 1e14, -1e20])
+def test_attention_scores_beyond_fp16_and_fp32_steps(count, dim, scale):
+    """Scores so large that fp32 numbers lie further apart than the weights'
+    range: the largest one takes all, as far as it stands out from a score's
+    error (2^-16 of scale sum |q||k| each).  Nothing overflows."""
+    case = Case([700], [count], 1, dim, page=16, seed=count, junk=True)
+    for dtype in (torch.float16, torch.bfloat16):
+        q = case.queries(2, dim, dtype)
+        out, lse = (f64(x) for x in case.cache.attention(q, case.batch, scale=scale, return_log_sum=True))
+        k, v = case.sequence(0, 0)[:, 0], case.sequence(0, 1)[:, 0]
+        assert np.isfinite(out).all() and np.isfinite(lse).all()
+        clear = 0
+        for i in range(count):
+            n = 700 - count + i + 1
+            for h in range(2):
+                s = scale * (k[:n] @ f64(q[i, h]))
+                d = 2.0**-16 * abs(scale) * (np.abs(k[:n]) @ np.abs(f64(q[i, h]))).max()
+                assert abs(lse[i, h] - s.max()) <= d + 2.0**-20 * abs(s.max()) + np.log(n)
+                assert (np.abs(out[i, h]) <= np.abs(v[:n]).max(0) * (1 + 2.0**-7)).all()
+                best, second = np.argsort(s)[-1], np.sort(s)[-2]
+                if s[best] - second > 2 * d + 60:  # the others weigh less than e^-60 together with n of them
+                    clear += 1
+                    tol = (U[dtype] + 2.0**-11 + 2.0**-20) * np.abs(v[best]) + 2.0**-25
+                    assert (np.abs(out[i, h] - v[best]) <= tol).all()
+        assert clear > count // 2
+    assert device_error() == 0
+
+
+@pytest.mark.parametrize("count", [1, 200])
+@pytest.mark.parametrize("scale", [0.0, -0.3, 3.0, 1e9])
+def test_attention_of_scales(count, scale):
+    """A scale of zero (the mean of what a row sees), a negative one; equal
+    scores of any size."""
+    case = Case([300, 31], [count, 1], 2, 64, page=16, seed=count, junk=True)
+    q = case.queries(8, 64, torch.bfloat16)
+    if scale > 1:  # all keys of a head alike
+        codes, scales = case.arrays[0]
+        codes[:], scales[:] = codes[:1, :, :1], 1
+        case.cache.k_codes.copy_(torch.from_numpy(ko.pack(codes)))
+        case.cache.k_scales.copy_(torch.from_numpy(scales))
+    out, lse = case.cache.attention(q, case.batch, scale=scale, return_log_sum=True)
+    seen = [(b, np.arange(p + 1)) for b, (n, c) in enumerate(zip(case.lengths, case.counts)) for p in range(n - c, n)]
+    if scale > 1:
+        mean = np.stack([case.sequence(b, 1)[i].mean(0) for b, i in seen]).repeat(4, 1)
+        spread = np.stack([np.abs(case.sequence(b, 1)[i]).mean(0) for b, i in seen]).repeat(4, 1)
+        assert (np.abs(f64(out) - mean) <= 2.0**-8 * np.abs(mean) + (2.0**-11 + 2.0**-14) * spread).all()
+    else:
+        check_seen(case, q, out, lse, seen, scale=scale)
+    assert device_error() == 0
