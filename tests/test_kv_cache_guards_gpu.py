@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import kv4_oracle as ko
-from test_kv_cache_gpu import TINY, U, Case, _device, device_error, f64  # noqa: F401 (_device: a fixture)
+from test_kv_cache_gpu import (TINY, U, Case, _device, append_reference, device_error, f64,  # noqa: F401 (a fixture)
+                               places)
 
 pytestmark = pytest.mark.gpu
 
@@ -430,4 +431,58 @@ def test_attention_of_scales(count, scale):
         assert (np.abs(f64(out) - mean) <= 2.0**-8 * np.abs(mean) + (2.0**-11 + 2.0**-14) * spread).all()
     else:
         check_seen(case, q, out, lse, seen, scale=scale)
+    assert device_error() == 0
+
+
+@pytest.mark.parametrize("sequences", [33, 129, 257, 300, 513, 600, 2048])
+def test_batches_of_many_sequences(sequences):
+    """Sums over the sequences that take more than one pass: append, read and
+    attention of many short ones, empty ones and some prompts among them."""
+    from openquant_b200.kv_cache import rotary_table
+
+    rng = np.random.default_rng(sequences)
+    counts = rng.integers(0, 3, sequences)
+    counts[rng.integers(0, sequences, 5)] = 40  # 80 query rows: the prompt kernel
+    counts[-1] = 45
+    lengths = np.where(counts > 0, counts + rng.integers(0, 30, sequences), rng.integers(0, 2, sequences) * 7)
+    case = Case([int(n) for n in lengths], [int(n) for n in counts], 1, 64, page=16, seed=sequences, junk=True)
+    t = case.tokens
+    pad = 3
+    q, k, v = (torch.randn(t + pad, h, 64, device="cuda").half() for h in (2, 1, 1))
+    table = rotary_table(128, 64)
+    page, row, pos = places(case)
+    turned = case.cache.append(k, v, case.batch, q=q, table=table)
+    want = ko.rotate(f64(q[:t]).astype(np.float32), table.cpu().numpy(), pos)
+    assert torch.equal(turned[:t].cpu(), torch.from_numpy(want).half())
+    refs = append_reference(case, k[:t], v[:t], 32, table, pos, False)
+    for (codes, scales), (new_codes, new_scales) in zip(case.arrays, refs):
+        codes[page, :, row], scales[page, :, row] = new_codes, new_scales
+    for x, (codes, scales) in zip(case.cache.read(case.batch, t + pad), refs):
+        assert np.array_equal(f64(x[:t]), ko.values(codes, scales)) and not x[t:].any()
+    out, lse = case.cache.attention(turned, case.batch, return_log_sum=True)
+    case.check(turned[:t], out[:t], lse[:t])
+    assert not out[t:].any() and (lse[t:] == float("-inf")).all()
+
+
+@pytest.mark.parametrize("dim, heads, length, count, window, bad", [
+    (128, 8, 300, 300, 0, 100), (64, 4, 700, 200, 0, 690), (128, 4, 5003, 40, 0, 4990),   # (cut over its tokens)
+    (64, 2, 5003, 64, 20, 4950), (64, 2, 5003, 64, 3000, 1960), (128, 1, 300, 300, 50, 128),
+])
+def test_prompts_over_a_key_that_is_not_finite(dim, heads, length, count, window, bad):
+    """Rows that see it are NaN, the others are whole."""
+    case = Case([length], [count], 1, dim, page=32, seed=dim, junk=True)
+    where = case.table[0, bad // 32], 0, bad % 32
+    for codes, scales, value in ((case.cache.k_codes, case.cache.k_scales, float("nan")),
+                                 (case.cache.v_codes, case.cache.v_scales, 1.0)):
+        codes[where], scales[where] = 0, value
+    q = case.queries(heads, dim, torch.bfloat16)
+    out, lse = case.cache.attention(q, case.batch, window=window, return_log_sum=True)
+    places_of = range(length - count, length)
+    sees = [p >= bad and (window == 0 or bad > p - window) for p in places_of]
+    assert any(sees) and not all(sees)
+    assert np.array_equal(np.isnan(f64(out)), np.broadcast_to(np.array(sees)[:, None, None], out.shape))
+    assert np.array_equal(np.isnan(f64(lse)), np.broadcast_to(np.array(sees)[:, None], lse.shape))
+    keep = [i for i, s in enumerate(sees) if not s]
+    check_seen(case, q[keep], out[keep], lse[keep],
+               [(0, np.arange(max(places_of[i] + 1 - window, 0) if window else 0, places_of[i] + 1)) for i in keep])
     assert device_error() == 0
