@@ -899,7 +899,8 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     OQ_REQUIRE(aligned(out, 16) && aligned(workspace, 16), "kv4_attention: out and workspace must be 16-byte aligned");
     OQ_REQUIRE(window >= 0, "kv4_attention: window must not be negative");
     OQ_REQUIRE((flags & ~OQ_KV4_NOT_CAUSAL) == 0, "kv4_attention: unknown flags");
-    OQ_REQUIRE(scale == scale && scale - scale == 0.0f, "kv4_attention: scale must be finite");
+    const float f = scale * 1.4426950408889634f;
+    OQ_REQUIRE(f - f == 0.0f, "kv4_attention: scale must be finite, times log2 e too");
     OQ_REQUIRE((int64_t)ws_bytes >= oq_kv4_attention_workspace_bytes(cache, batch, q_heads, tokens),
                "kv4_attention: workspace too small");
     Args a = {};
@@ -920,7 +921,7 @@ extern "C" int oq_kv4_attention(const oq_kv4_cache *cache, const oq_kv4_batch *b
     a.max_tokens = batch->max_tokens;
     a.q_heads = q_heads;
     a.ratio = q_heads / cache->kv_heads;
-    a.f = scale * 1.4426950408889634f;
+    a.f = f;
     a.window = window < INT32_MAX ? window : 0;  // positions are below 2^31: no limit
     a.causal = (flags & OQ_KV4_NOT_CAUSAL) ? 0 : 1;
     a.parts = static_cast<float *>(workspace);

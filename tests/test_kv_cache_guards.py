@@ -86,3 +86,17 @@ def test_too_many_key_heads_are_refused_before_anything_is_launched():
     st = lib.oq_kv4_attention(ctypes.byref(cache), ctypes.byref(batch), p, nat.OQ_F16, heads, heads * 128, 128, p, None,
                               2, 1.0, 0, 0, p, 1 << 40, None)
     assert st == nat.OQ_ERR_INVALID and "key heads" in nat.last_error()
+
+
+def test_scales_whose_log2_factor_is_not_finite_are_refused():
+    import ctypes
+
+    from openquant_b200 import _native as nat, build, kv_cache as kc
+
+    build.build()
+    lib, p = nat.load(), 1 << 20
+    cache, batch = kc._Cache(p, p, p, p, 4, 16, 2, 128, 32), kc._Batch(p, p, None, 2, 2, 1)
+    for scale in (2.5e38, -3e38, math.inf, math.nan):
+        st = lib.oq_kv4_attention(ctypes.byref(cache), ctypes.byref(batch), p, nat.OQ_F16, 4, 512, 128, p, None, 2, scale,
+                                  0, 0, p, 1 << 30, None)
+        assert st == nat.OQ_ERR_INVALID and "finite" in nat.last_error()
