@@ -375,7 +375,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
             for (int i = 0; i < HD / 16; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[j][i][e] = 0.0f;
-            m[j][0] = m[j][1] = -1e30f;
+            m[j][0] = m[j][1] = kNone;
             most[j][0] = most[j][1] = -INFINITY;
             l[j][0] = l[j][1] = 0.0f;
         }
@@ -501,7 +501,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas<HD, NT>) stream_kernel(cons
                         const float mn = fmaxf(m[j][e], __fmul_rn(mx, f[j][e]) - kLift);
                         const float corr = ex2(m[j][e] - mn);
                         m[j][e] = mn;
-                        // (-1e30, nothing seen yet, passes kHuge too)
+                        // (kNone passes kHuge too)
                         most[j][e] = fabsf(mn) > kHuge ? -INFINITY : __fdividef(mn + kRaise, f[j][e]);
                         huge |= fabsf(mn) > kHuge;
                         l[j][e] *= corr;
@@ -690,7 +690,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a, int warps) {
         const int j = sl_i / (HD / 16), i = sl_i % (HD / 16), col = 8 * j + 2 * t4;
         const bool in = row0 + col < w.rows;
         // of the lane's two columns, over the parts so far
-        float m[2] = {-1e30f, -1e30f}, l[2] = {0.0f, 0.0f};
+        float m[2] = {kNone, kNone}, l[2] = {0.0f, 0.0f};
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (in) {
             constexpr int U = 8;  // parts in flight

@@ -14,6 +14,8 @@ constexpr float kRaise = 14.0f;  // and raised when a score passes it by more th
 // rounded: up to |s f| 2^-23 too much, and from 2^24 on p may pass fp16.
 constexpr float kHuge = 1048576.0f;
 
+constexpr float kNone = -3e38f;  // the maximum of no scores: finite, below what a score can be
+
 struct AttnArgs {
     const uint8_t *k_codes, *v_codes;
     const __half *k_scales, *v_scales;

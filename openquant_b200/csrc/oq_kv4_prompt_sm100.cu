@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
             const int all_low = a.window > 0 ? (int)max((int64_t)base + last / a.ratio + 1 - a.window, (int64_t)0) : 0;
             const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
             const uint32_t ts = tmem + quarter + kS + wg * kTok, to = tmem + quarter + kO + wg * HD;
-            float m = -1e30f;
+            float m = kNone;
             float lim = -INFINITY, fe = f;  // m is raised above it; what s is multiplied with in p
             float2 l2[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
             bool ok = __all_sync(0xffffffffu, wait(scanned, 0));
@@ -406,9 +406,9 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                             tmem_st_32x32b_x8(to + 8 * i, o);
                         }
                     }
-                    // (a row that has passed kHuge comes here with every block)
-                    const bool huge = m > -1e30f && fabsf(m) > kHuge;
-                    lim = m > -1e30f && !huge ? m + kRaise : -INFINITY;
+                    // (a row that has passed kHuge, or has kNone, comes here with every block)
+                    const bool huge = fabsf(m) > kHuge;
+                    lim = huge ? -INFINITY : m + kRaise;
                     fe = huge ? 1.0f : f;
                     if (huge) {
 #pragma unroll
@@ -709,7 +709,7 @@ __global__ void __launch_bounds__(kPromptRows) join_prompt_kernel(const __grid_c
     const int r = threadIdx.x, row = it.row0 + r;
     if (row >= it.rows) return;
     const float *src = a.parts + (int64_t)blockIdx.x * cuts * kPartFloats<HD> + r;
-    float m = -1e30f, l = 0.0f;
+    float m = kNone, l = 0.0f;
     for (int p = 0; p < it.parts; ++p) m = fmaxf(m, src[(int64_t)p * kPartFloats<HD>]);
     float4 o[4] = {};
 #pragma unroll 2

@@ -486,3 +486,23 @@ def test_prompts_over_a_key_that_is_not_finite(dim, heads, length, count, window
     check_seen(case, q[keep], out[keep], lse[keep],
                [(0, np.arange(max(places_of[i] + 1 - window, 0) if window else 0, places_of[i] + 1)) for i in keep])
     assert device_error() == 0
+
+
+@pytest.mark.parametrize("count", [1, 200])
+@pytest.mark.parametrize("sign", [-1.0, 1.0])
+def test_attention_of_bf16_queries_near_their_largest(count, sign):
+    """Scores of 1e32 and more of either sign, all equal: the mean of the values."""
+    case = Case([300, 31], [count, 1], 1, 64, page=16, seed=count, junk=True)
+    codes, scales = case.arrays[0]
+    codes[:], scales[:] = 5, 1
+    case.cache.k_codes.copy_(torch.from_numpy(ko.pack(codes)))
+    case.cache.k_scales.copy_(torch.from_numpy(scales))
+    q = torch.full((case.tokens, 4, 64), sign * 1e31, device="cuda").bfloat16()
+    out, lse = case.cache.attention(q, case.batch, return_log_sum=True)
+    seen = [(b, np.arange(p + 1)) for b, (n, c) in enumerate(zip(case.lengths, case.counts)) for p in range(n - c, n)]
+    mean = np.stack([case.sequence(b, 1)[i].mean(0) for b, i in seen])
+    spread = np.stack([np.abs(case.sequence(b, 1)[i]).mean(0) for b, i in seen])
+    assert (np.abs(f64(out) - mean) <= 2.0**-8 * np.abs(mean) + (2.0**-11 + 2.0**-14) * spread).all()
+    score = float(q[0, 0, 0]) * 5 * 64 * 0.125
+    assert (np.abs(f64(lse) - score) <= 2.0**-20 * abs(score)).all()
+    assert device_error() == 0
