@@ -16,7 +16,7 @@
 // Roles: warps 0-3 and 4-7 are the softmax of the two tiles (a thread a row),
 // warps 8-11 turn codes into fp16 tiles, warp 12 issues the products, warps
 // 13-15 see beforehand whether all pages are there (the softmax then looks up
-// no page: 165 us for 167 of ragged prompts with a word a block from the
+// no page: 165 us for 166 of ragged prompts with a word a block from the
 // dequantizing warps).  While one tile's softmax runs, the other tile's products do: P0 V, Q0 K', P1 V,
 // Q1 K', ...  The first half of a P is multiplied while the second is made.
 //
@@ -134,6 +134,9 @@ __device__ __forceinline__ bool wait(uint64_t *bar, uint32_t parity) {
 }
 
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// The lowest n bits of a word; n may be below 0 or above 32.
+__device__ __forceinline__ uint32_t ones(int n) { return n >= 32 ? 0xFFFFFFFFu : (1u << max(n, 0)) - 1; }
 
 // Byte offset of the 16-byte chunk `c` (eight elements) of row r.
 template <int PANEL>
@@ -368,16 +371,21 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                 if (holes || t0 + kTok > all_vis || t0 < all_low) {
                     const int e0 = (int)min(max(low - t0, (int64_t)0), (int64_t)kTok);
                     const int e1 = (int)min(max(vis - t0, (int64_t)0), (int64_t)kTok);
-#pragma unroll
-                    for (int i = 0; i < kTok; ++i)
-                        if (i < e0 || i >= e1) s[i >> 5][i & 31] = 0xff800000u;
+                    uint32_t gone = 0;  // bit i: tokens 16 i .. of the block have no page
                     if (holes) {
-#pragma unroll
+#pragma unroll 1
                         for (int i = 0; i < kTok / 16; ++i)
-                            if (t0 + 16 * i < hi && page_of(t0 + 16 * i) < 0) {
+                            if (t0 + 16 * i < hi && page_of(t0 + 16 * i) < 0) gone |= 1u << i;
+                    }
+                    // As words of 32 tokens, not by comparisons of each: ragged prompts 167 us
+                    // with those (and two more loops' code for the pages), 156 with words.
 #pragma unroll
-                                for (int e = 0; e < 16; ++e) s[i >> 1][(i & 1) * 16 + e] = 0xff800000u;
-                            }
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t seen = ones(e1 - 32 * w) & ~ones(e0 - 32 * w);
+                        const uint32_t hide = ~seen | (gone >> 2 * w & 1) * 0xFFFFu | (gone >> (2 * w + 1) & 1) * 0xFFFF0000u;
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            if (hide >> e & 1) s[w][e] = 0xff800000u;
                     }
                 }
                 float mx[4];
@@ -410,12 +418,13 @@ __global__ void __launch_bounds__(kThreads, 1) prompt_kernel(const __grid_consta
                     const bool huge = fabsf(m) > kHuge;
                     lim = huge ? -INFINITY : m + kRaise;
                     fe = huge ? 1.0f : f;
-                    if (huge) {
+                    if (__any_sync(0xffffffffu, huge)) {
+                        const float fm = huge ? f : 1.0f;
 #pragma unroll
                         for (int i = 0; i < kTok; i += 2) {
                             const float2 x = __fmul2_rn(make_float2(__uint_as_float(s[i >> 5][i & 31]),
                                                                     __uint_as_float(s[i >> 5][(i & 31) + 1])),
-                                                        make_float2(f, f));
+                                                        make_float2(fm, fm));
                             s[i >> 5][i & 31] = __float_as_uint(x.x);
                             s[i >> 5][(i & 31) + 1] = __float_as_uint(x.y);
                         }
