@@ -111,8 +111,9 @@ OQ_API int oq_device_count(void);
  * error word of the library's pipelined kernels: *code = 0 when none, 1 when
  * a kernel gave up waiting on one of its internal pipeline barriers (it then
  * returned early, its outputs are undefined), 2 when oq_peer_barrier gave
- * up waiting for a peer GPU, 3 when a 4-bit cache kernel met a page number
- * or a position outside its arrays.  No reference counterpart: the reference's
+ * up waiting for a peer GPU, 3 when a 4-bit cache kernel met a page number,
+ * a position or a sequence's starts outside their arrays, or more tokens than
+ * max_tokens (what they stand for was left out).  No reference counterpart: the reference's
  * Triton kernel has no internal waits.
  */
 OQ_API int oq_take_device_error(int32_t *code);
@@ -451,7 +452,8 @@ typedef struct {
  * All arrays int32, on the device.
  * A page number outside the cache, a position outside the page table or the
  * rotary table is not followed: the access is left out and the device error
- * becomes 3 (oq_take_device_error). */
+ * becomes 3 (oq_take_device_error).  Attention treats such tokens as masked;
+ * positions are those of lengths[b], within the table or not. */
 typedef struct {
     const int32_t *page_table;
     const int32_t *lengths;
@@ -494,7 +496,9 @@ OQ_API int oq_rotary(const void *x, void *y, int dtype, int64_t tokens,
  * rotated into q_out (which may be q).  k, v [tokens][kv_heads][head_dim] and q
  * [tokens][q_heads][head_dim] are fp16 or bf16, strides in elements, a head
  * contiguous.  positions (int32 / int64 [tokens]) replaces the tokens' places
- * in their sequences for the rotation only; NULL: those places. */
+ * in their sequences for the rotation only; NULL: those places.  A token whose
+ * position is outside the rotary table is not written, neither to the cache
+ * nor to q_out. */
 OQ_API int oq_kv4_append(const oq_kv4_cache *cache, const oq_kv4_batch *batch,
                          const void *q, void *q_out, int q_heads,
                          int64_t q_token_stride, int64_t q_head_stride,

@@ -19,9 +19,9 @@
 //
 // What bounds it.  The cache has to be read once: 144 bytes a token and key
 // head (head_dim 128, groups of 32).  64 ragged sequences of 333 to 8192 tokens
-// (64 query, 8 key heads): 81.5 us, 60 % of the measured copy rate, DRAM traffic
+// (64 query, 8 key heads): 81.6 us, 59 % of the measured copy rate, DRAM traffic
 // 1.00 x the cache's bytes; two of 100003 and 131071 tokens (groups of 64) 65
-// us, 60 %.  ncu: instruction issue 61 % of the cycles with 12 warps an SM, 22
+// us, 59 %.  ncu: instruction issue 62 % of the cycles with 12 warps an SM, 22
 // instructions a token and key head, most of them the unpacking (9 for eight
 // codes, and 4 more for the scale of V); no bank conflicts, tensor pipe 22 %.
 // So it is bound by issue and by the latency of what each warp does in turn.

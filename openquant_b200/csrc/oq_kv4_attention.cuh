@@ -12,6 +12,8 @@ constexpr float kRaise = 14.0f;  // and raised when a score passes it by more th
 // Scores beyond this (log2) are rounded to fp32 before the maximum is taken off.
 // One fused operation would take the exact product s f less a maximum that was
 // rounded: up to |s f| 2^-23 too much, and from 2^24 on p may pass fp16.
+// (Beyond 2^26 fp32 numbers lie further apart than kLift: the largest p of a
+// row is then 1 to 2^8.)
 constexpr float kHuge = 1048576.0f;
 
 constexpr float kNone = -3e38f;  // the maximum of no scores: finite, below what a score can be

@@ -17,8 +17,9 @@
 // warps 8-11 turn codes into fp16 tiles, warp 12 issues the products, warps
 // 13-15 see beforehand whether all pages are there (the softmax then looks up
 // no page: 165 us for 166 of ragged prompts with a word a block from the
-// dequantizing warps).  While one tile's softmax runs, the other tile's products do: P0 V, Q0 K', P1 V,
-// Q1 K', ...  The first half of a P is multiplied while the second is made.
+// dequantizing warps).  While one tile's softmax runs, the other tile's
+// products do: P0 V, Q0 K', P1 V, Q1 K', ...  The first half of a P is
+// multiplied while the second is made.
 //
 // What bounds it.  For 4096 queries over 32768 tokens (64 query and 8 key
 // heads, bf16): 3.11 ms, 1.32 PFLOP/s, 80 % of the measured dense bf16 rate,
@@ -97,8 +98,8 @@ __device__ __forceinline__ void regs_dec() {
 
 // One lane of a converged warp, in a form in which the compiler knows that the
 // warp is converged: it then keeps the products' operands in uniform registers.
-// (Issued behind `lane == 0` a product took 115 cycles instead of 89, in a
-// block that needs 48 of them.)
+// (Issued behind `lane == 0` a product took 115 cycles instead of 89; a block
+// of two tiles needs 2 (head_dim / 16 + 8) of them.)
 __device__ __forceinline__ bool elect_one() {
     uint32_t v;
     asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(v));

@@ -47,8 +47,8 @@ def take_device_error():
     """Reads and clears the library's device error word of the current GPU,
     after the work on it has ended: 0, or what a kernel met first -- 1 gave up
     waiting inside a kernel (its outputs are undefined), 2 for a peer GPU, 3 a
-    page number, position or start of a sequence outside its array (the access
-    was left out)."""
+    page number, a position or a sequence's starts outside their arrays, or more
+    tokens than max_tokens (what they stand for was left out)."""
     nat.require_device()
     code = ctypes.c_int32()
     nat.check(nat.load().oq_take_device_error(ctypes.byref(code)))
@@ -415,7 +415,8 @@ class Int4KVCache:
         their place in the sequence, or by `positions` ([tokens], int32 or
         int64) where given; q [tokens, heads, head_dim] is rotated likewise and
         returned in q's dtype (q_out, which may be q, takes it; None without
-        q).  One kernel."""
+        q).  A token whose position is outside the table is not written,
+        neither to the cache nor to q's output.  One kernel."""
         tokens, heads, dim = _heads(k, "k")
         if heads != self.kv_heads or dim != self.head_dim:
             raise ValueError("k must have the cache's kv_heads and head_dim")
